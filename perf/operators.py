@@ -253,7 +253,8 @@ def _plain_select(logits, scores, beams, live):
     if live is not None:
         x = x.masked_fill(torch.arange(outputs, device="cuda") >= live[:, None, None], -math.inf)
     top = x.amax(-1, keepdim=True)
-    total = torch.log(torch.exp(x - top).sum(-1, keepdim=True)) + top
+    x = x - top
+    total = torch.log(torch.exp(x).sum(-1, keepdim=True))
     cand = (x + (scores.double()[..., None] - total)).float().reshape(groups, into * outputs)
     cand = torch.where(cand.isnan(), torch.full_like(cand, -math.inf), cand) + 0.0
     bits = cand.view(torch.int32).long()
