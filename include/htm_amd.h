@@ -448,6 +448,95 @@ int htm_cls_export_state(htm_classifier* cls, int32_t region, int32_t stream_beg
 int htm_cls_import_state(htm_classifier* cls, int32_t region, int32_t stream_begin, int32_t n, const void* h_src,
                          size_t bytes);
 
+/* ---- 4-bit read-out ---------------------------------------------------------
+ * A frozen linear map from cells (or columns) to buckets, 4 bits a weight and
+ * one bfloat16 scale per `group` neighbouring buckets: the SDRClassifier's
+ * product (above) at 1/15 of its float64 matrices' bytes, so that a fleet's
+ * streams can answer too.
+ *   y[r][h][o] = sum_i x[r][i] * scale[m][i][h][o / group] * (code[m][i][h][o] - 8)
+ * r = 0..n_rows-1, m = r / (n_rows / n_models): consecutive rows share a matrix
+ * (a stream's beams; all rows when n_models is 1).  Sums in float32.
+ * Records: uint8 [n_models][n_inputs][htm_q4_record_bytes], one input's weights:
+ * per head the codes of its outputs (padded to a multiple of 32; the lower half
+ * of a byte first), then per head ceil(padded / group) scales; padding is
+ * ignored.  Base address and d_x / d_pattern / d_out as the element type asks,
+ * records 16-byte aligned. */
+typedef struct {
+    int32_t n_models;
+    int32_t n_inputs;   /* 1..65536; patterns need a multiple of 32 */
+    int32_t n_heads;    /* 1..64 (look-ahead steps) */
+    int32_t n_outputs;  /* 1..65536 per head; n_heads * padded outputs <= 1048576 */
+    int32_t group;      /* 32, 64 or 128 */
+} htm_q4_shape;
+#define HTM_T_F32 0
+#define HTM_T_F64 1
+#define HTM_T_F16 2
+#define HTM_T_BF16 3
+/* Bytes of one input's record, a multiple of 64 (0: invalid shape). */
+size_t htm_q4_record_bytes(const htm_q4_shape* shape);
+/* Quantise d_weights (HTM_T_F32 / HTM_T_F64; element (m, i, h, o) at m * model_stride +
+ * i * input_stride + h * head_stride + o) into d_records: scale = bfloat16(max|w| of
+ * the group / 7), code = 8 + w / scale rounded to nearest even, within 1..15; a zero
+ * stays exactly zero.  *d_bad (DEVICE int32, zeroed by the caller) is set to 1 if a
+ * weight is infinite or NaN (its code is then meaningless). */
+int htm_q4_quantise(const htm_q4_shape* shape, const void* d_weights, int32_t dtype, int64_t model_stride,
+                    int64_t input_stride, int64_t head_stride, void* d_records, int32_t* d_bad, void* stream);
+/* The same from a classifier's streams [stream_begin, stream_begin + n_models) and
+ * the n_heads of its steps from the step_begin-th on (n_inputs and n_outputs as the
+ * classifier's); d_live (DEVICE int32 [n_models]) receives the streams' live bucket
+ * counts (maxBucketIdx + 1). */
+int htm_cls_quantise(const htm_classifier* cls, int32_t stream_begin, int32_t step_begin, const htm_q4_shape* shape,
+                     void* d_records, int32_t* d_live, int32_t* d_bad, void* stream);
+/* y for word bitmaps: d_pattern DEVICE uint32, row r at r * pattern_stride words
+ * (n_inputs / 32 of them used; bit b of word w is input 32 w + b).  d_out: float
+ * [n_rows][n_heads][n_outputs]. */
+int htm_q4_logits(const htm_q4_shape* shape, const void* d_records, const uint32_t* d_pattern, int64_t pattern_stride,
+                  int32_t n_rows, float* d_out, void* stream);
+/* softmax of y over each head's first live outputs, 0 above (n_outputs <= 1024).
+ * d_live: DEVICE int32 [n_models], clamped to 0..n_outputs; NULL: all. */
+int htm_q4_probabilities(const htm_q4_shape* shape, const void* d_records, const uint32_t* d_pattern,
+                         int64_t pattern_stride, const int32_t* d_live, int32_t n_rows, float* d_out, void* stream);
+/* y for vectors of numbers (HTM_T_F32 / F16 / BF16, row r at r * x_stride elements).
+ * d_work: DEVICE scratch of htm_q4_work_bytes (may be NULL when that is 0), not
+ * shared with a call that may run at the same time. */
+size_t htm_q4_work_bytes(const htm_q4_shape* shape, int32_t n_rows);
+int htm_q4_matvec(const htm_q4_shape* shape, const void* d_records, const void* d_x, int32_t dtype, int64_t x_stride,
+                  int32_t n_rows, float* d_out, void* d_work, size_t work_bytes, void* stream);
+
+/* ---- beams -------------------------------------------------------------------
+ * A forecast that follows several continuations of every stream at once.
+ * htm_beam_select: of the beams_in * n_outputs continuations of each group the
+ * best n_beams by score, ties by the lower place w * n_outputs + o:
+ *   s(w, o) = float32((x[w][o] - m) + (score[w] - log(sum_{o' < live} exp(x[w][o'] - m)))),
+ * m the beam's largest live logit (everything in float64 up to that one rounding).  A continuation whose s is
+ * -infinity or NaN, or with o >= live, is never taken; a slot left over gets
+ * score -infinity, bucket -1 and parent min(slot, beams_in - 1).
+ * d_logits (HTM_T_F32 / F16 / BF16): element (g, w, o) at g * group_stride +
+ * w * beam_stride + o; d_scores float [n_groups][beams_in]; d_live int32
+ * [n_groups], clamped to 0..n_outputs, or NULL.  Out: float / int32 / int32
+ * [n_groups][n_beams], best first.  1 <= beams_in, n_beams <= 64, beams_in *
+ * n_outputs < 2^31.  d_work as for htm_q4_matvec. */
+size_t htm_beam_work_bytes(int32_t n_groups, int32_t beams_in, int32_t n_beams, int32_t n_outputs);
+int htm_beam_select(const void* d_logits, int32_t dtype, int64_t group_stride, int64_t beam_stride,
+                    const float* d_scores, const int32_t* d_live, int32_t n_groups, int32_t beams_in, int32_t n_beams,
+                    int32_t n_outputs, float* d_out_scores, int32_t* d_out_parent, int32_t* d_out_bucket,
+                    void* d_work, size_t work_bytes, void* stream);
+/* Row (g, w) of every destination buffer becomes row (g, d_parent[g][w]) of its
+ * source: n_buffers (1..32) buffers of n_groups * n_beams rows of row_bytes[k] bytes.
+ * d_dst[k] == d_src[k] reorders in place (the rows' old contents are read first);
+ * other overlaps are refused.  A parent outside 0..n_beams-1 counts as w itself. */
+#define HTM_BEAM_BUFFERS 32
+int htm_beam_reorder(int32_t n_buffers, const void* const* d_src, void* const* d_dst, const size_t* row_bytes,
+                     const int32_t* d_parent, int32_t n_groups, int32_t n_beams, void* stream);
+/* The same for every per-stream state and output of a fleet (htm_create_fleet), in
+ * place: stream g * n_beams + w goes on as its parent d_parent[g][w] would have.
+ * n_streams must be a multiple of n_beams. */
+int htm_reorder_streams(htm_engine* eng, const int32_t* d_parent, int32_t n_beams, void* stream);
+/* Stream s of fleet dst goes on as stream d_index[s] (DEVICE int32 [n_streams of
+ * dst], 0..n_streams of src - 1; others leave s as it is) of fleet src: a fork.
+ * Both are fleets of one model, alike in configuration, on one device; dst != src. */
+int htm_copy_streams(htm_engine* dst, htm_engine* src, const int32_t* d_index, void* stream);
+
 const char* htm_last_error(void);
 int32_t htm_abi_version(void);
 /* How the library was built: "<unit> <optimisation level>;..." for every

@@ -7,7 +7,9 @@ from . import _lib
 from ._lib import HtmConfig, HtmError, build, default_config
 from .engine import HTMEngine
 from . import classifier, fleet, harness, ingest
+from .beam import beam_reorder, beam_select
 from .harness import AnomalyLikelihood, SLOHarness
 from .network import BatchRecordStream, MultiEncoder, Network, ScalarEncoder
+from .readout import Readout4
 
-__all__ = ["AnomalyLikelihood", "SLOHarness", "HTMEngine", "Network", "BatchRecordStream", "MultiEncoder", "ScalarEncoder", "HtmConfig", "HtmError", "build", "default_config", "_lib"]
+__all__ = ["AnomalyLikelihood", "SLOHarness", "HTMEngine", "Network", "BatchRecordStream", "MultiEncoder", "ScalarEncoder", "HtmConfig", "HtmError", "Readout4", "beam_reorder", "beam_select", "build", "default_config", "_lib"]

@@ -110,6 +110,12 @@ class TmUpdate(ctypes.Structure):
                 ("new_src", ctypes.c_uint16 * 32)]
 
 
+class Q4Shape(ctypes.Structure):
+    """Mirror of htm_q4_shape."""
+    _fields_ = [("n_models", ctypes.c_int32), ("n_inputs", ctypes.c_int32), ("n_heads", ctypes.c_int32),
+                ("n_outputs", ctypes.c_int32), ("group", ctypes.c_int32)]
+
+
 EXPORTED = [
     "htm_default_config", "htm_create", "htm_destroy", "htm_set_learning", "htm_set_option", "htm_status",
     "htm_step", "htm_run", "htm_step_sdr", "htm_run_sdr", "htm_get_output", "htm_output_bytes", "htm_state_bytes", "htm_export_state",
@@ -119,7 +125,9 @@ EXPORTED = [
     "htm_slo_create", "htm_slo_destroy", "htm_slo_record", "htm_slo_stats", "htm_create_fleet", "htm_is_fleet", "htm_flush",
     "htm_likelihood_create", "htm_likelihood_destroy", "htm_likelihood_step",
     "htm_cls_create", "htm_cls_destroy", "htm_cls_compute", "htm_cls_status", "htm_cls_state_bytes",
-    "htm_cls_export_state", "htm_cls_import_state",
+    "htm_cls_export_state", "htm_cls_import_state", "htm_cls_quantise",
+    "htm_q4_record_bytes", "htm_q4_quantise", "htm_q4_logits", "htm_q4_probabilities", "htm_q4_work_bytes", "htm_q4_matvec",
+    "htm_beam_work_bytes", "htm_beam_select", "htm_beam_reorder", "htm_reorder_streams", "htm_copy_streams",
 ]
 
 _lib = None
@@ -209,6 +217,22 @@ def lib():
     L.htm_slo_destroy.argtypes = [vp]
     L.htm_slo_record.argtypes = [vp, vp, i32, vp, vp, vp, vp]
     L.htm_slo_stats.argtypes = [vp, P(ctypes.c_int64), vp]
+    i64 = ctypes.c_int64
+    L.htm_cls_quantise.argtypes = [vp, i32, i32, vp, vp, vp, vp, vp]
+    L.htm_q4_record_bytes.argtypes = [vp]
+    L.htm_q4_record_bytes.restype = sz
+    L.htm_q4_quantise.argtypes = [vp, vp, i32, i64, i64, i64, vp, vp, vp]
+    L.htm_q4_logits.argtypes = [vp, vp, vp, i64, i32, vp, vp]
+    L.htm_q4_probabilities.argtypes = [vp, vp, vp, i64, vp, i32, vp, vp]
+    L.htm_q4_work_bytes.argtypes = [vp, i32]
+    L.htm_q4_work_bytes.restype = sz
+    L.htm_q4_matvec.argtypes = [vp, vp, vp, i32, i64, i32, vp, vp, sz, vp]
+    L.htm_beam_work_bytes.argtypes = [i32, i32, i32, i32]
+    L.htm_beam_work_bytes.restype = sz
+    L.htm_beam_select.argtypes = [vp, i32, i64, i64, vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, sz, vp]
+    L.htm_beam_reorder.argtypes = [i32, vp, vp, vp, vp, i32, i32, vp]
+    L.htm_reorder_streams.argtypes = [vp, vp, i32, vp]
+    L.htm_copy_streams.argtypes = [vp, vp, vp, vp]
     _lib = L
     return L
 

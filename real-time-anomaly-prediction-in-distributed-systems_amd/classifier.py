@@ -91,6 +91,14 @@ class SDRClassifier:
         self._keep = (p, b, v)
         return self.probabilities, self.actual_values
 
+    def readout4(self, s0: int = 0, n: int | None = None, group: int = 32, steps=None):
+        """The present weights of streams [s0, s0 + n) in 4 bits: a frozen
+        `Readout4` that answers `probabilities` for those streams (or, from
+        one stream, for a fleet that shares its model).  steps: neighbouring
+        entries of this classifier's to take (default: all)."""
+        from .readout import Readout4
+        return Readout4.from_classifier(self, s0, n, group, steps)
+
     def status(self) -> int:
         f = ctypes.c_int32()
         check(self._L.htm_cls_status(self.h, ctypes.byref(f)))

@@ -32,6 +32,7 @@
 #include <stdint.h>
 
 #include "htm_dev.h"
+#include "q4_dev.h"
 
 #define CLS_NT 256
 #define CLS_MAX_STEPS 16
@@ -335,6 +336,27 @@ int htm_cls_compute(htm_classifier* h, const uint32_t* d_pattern, const int32_t*
     hipLaunchKernelGGL(cls_step_kernel, dim3(h->b.n, h->b.nsteps), dim3(CLS_NT), 0, st, h->b, infer ? 1 : 0,
                        d_probabilities);
     return hipGetLastError() == hipSuccess ? HTM_OK : htm_fail(HTM_E_HIP, "%s: HIP launch/sync failed", __func__);
+}
+
+// maxBucketIdx + 1 of streams [s0, s0 + n)
+__global__ void cls_live_kernel(const ClsState* st, int n, int nb, int32_t* live) {
+    const int s = blockIdx.x * blockDim.x + threadIdx.x;
+    if (s < n) live[s] = min(st[s].max_bucket + 1, nb);
+}
+
+int htm_cls_quantise(const htm_classifier* h, int32_t s0, int32_t y0, const htm_q4_shape* shape, void* d_records,
+                     int32_t* d_live, int32_t* d_bad, void* stream) {
+    Q4Dims d;
+    if (int r = q4_dims(shape, __func__, &d)) return r;
+    if (!h || !d_records || (uintptr_t)d_records % 16 || !d_live || !d_bad || s0 < 0 || (int64_t)s0 + d.nm > h->b.n ||
+        y0 < 0 || (int64_t)y0 + d.nh > h->b.nsteps || d.ni != h->b.ncells || d.no != h->b.nb)
+        return htm_fail(HTM_E_INVALID, "%s: invalid argument", __func__);
+    const ClsBufs& b = h->b;
+    const int64_t per = (int64_t)b.ncells * b.nb;
+    hipLaunchKernelGGL(cls_live_kernel, dim3((d.nm + 255) / 256), dim3(256), 0, (hipStream_t)stream, b.st + s0, d.nm,
+                       b.nb, d_live);
+    return q4_quantise_launch(d, b.w + ((int64_t)s0 * b.nsteps + y0) * per, HTM_T_F64, b.nsteps * per, b.nb, per, d_records,
+                              d_bad, (hipStream_t)stream);
 }
 
 static int cls_region(const htm_classifier* h, int32_t region, void** base, size_t* per) {

@@ -17,6 +17,7 @@
 #include <string>
 #include <vector>
 
+#include "beam_dev.h"
 #include "htm_dev.h"
 
 static thread_local std::string g_err;
@@ -1639,6 +1640,77 @@ int htm_create_fleet(const htm_engine* model, int32_t model_stream, int32_t n_st
     e->sp_learn = e->tm_learn = 0;
     *out = e;
     return HTM_OK;
+}
+
+// The per-stream state and outputs of a fleet's streams (the model's regions
+// are shared): what a stream needs to go on as another would have, and what
+// htm_get_output reads.  The packed colConfidence always (the next step reads
+// it wherever its flag word says so, also after it was made dense), the dense
+// one unless a step has left it behind.
+static int stream_rows(const htm_engine* e, RowMoves& m) {
+    const DevCfg& d = e->dc;
+    m.n = 0;
+    auto add = [&](const void* p, size_t bytes) {
+        if (!p || !bytes) return;
+        m.src[m.n] = (const uint8_t*)p;
+        m.dst[m.n] = (uint8_t*)const_cast<void*>(p);
+        m.bytes[m.n++] = bytes;
+    };
+    for (int id = 1; id <= HTM_ST_COUNT; id++) {
+        const Region& r = e->regions[id];
+        if (!r.model && id != HTM_ST_TM_COLCONF) add(r.base, r.per_stream);
+    }
+    add(e->tm.colnz, ((size_t)d.nw + 1) * 4);
+    add(e->tm.colval, (size_t)d.ncol * 4);
+    if (!e->conf_packed) add(e->tm.colconf, (size_t)d.ncol * 4);
+    add(e->sp.act, HTM_MAXACT * 2);
+    add(e->sp.nact, 4);
+    add(e->sp.err, 4);
+    add(e->sp.enc_bucket, 16);
+    if (e->keep_overlaps) add(e->sp.overlaps, (size_t)d.ncol * 4);
+    if (e->keep_prev) add(e->tm.prev_pred, (size_t)d.ncol);
+    return HTM_OK;
+}
+
+// A flush beside the steps reads its streams' headers: rows move after it.  The
+// log of deferred writes stays where it is -- its entries name cells and the
+// shared model's records, whichever stream logged them.
+static int after_flush(htm_engine* e, hipStream_t st) {
+    if (e->flush_pending) HIP_TRY(hipStreamWaitEvent(st, e->ev_flushed, 0));
+    return HTM_OK;
+}
+
+int htm_reorder_streams(htm_engine* e, const int32_t* d_parent, int32_t n_beams, void* stream) {
+    if (!e || !d_parent) return htm_fail(HTM_E_INVALID, "bad arguments");
+    if (!e->fleet) return htm_fail(HTM_E_STATE, "streams of an ordinary engine have models of their own: reorder a fleet");
+    if (n_beams < 1 || n_beams > 64 || e->n % n_beams)
+        return htm_fail(HTM_E_INVALID, "n_beams must be 1..64 and divide the %d streams", e->n);
+    if (int r = after_flush(e, (hipStream_t)stream)) return r;
+    RowMoves m;
+    stream_rows(e, m);
+    return rows_move(m, d_parent, e->n, n_beams, e->n, (hipStream_t)stream);
+}
+
+int htm_copy_streams(htm_engine* dst, htm_engine* src, const int32_t* d_index, void* stream) {
+    if (!dst || !src || !d_index || dst == src) return htm_fail(HTM_E_INVALID, "bad arguments");
+    if (!dst->fleet || !src->fleet) return htm_fail(HTM_E_STATE, "streams are copied between fleets of one model");
+    if (dst->device != src->device) return htm_fail(HTM_E_INVALID, "the fleets are on devices %d and %d", dst->device, src->device);
+    if (std::memcmp(&dst->cfg, &src->cfg, sizeof(htm_config)))
+        return htm_fail(HTM_E_INVALID, "the fleets' configurations differ");
+    if (dst->keep_overlaps != src->keep_overlaps || dst->keep_prev != src->keep_prev)
+        return htm_fail(HTM_E_INVALID, "the fleets retain different outputs (HTM_OPT_KEEP_*)");
+    hipStream_t st = (hipStream_t)stream;
+    if (int r = after_flush(dst, st)) return r;
+    // (one of the two stepped since its colConfidence was last made dense)
+    if (dst->conf_packed != src->conf_packed) {
+        if (int r = densify_conf(dst, st)) return r;
+        if (int r = densify_conf(src, st)) return r;
+    }
+    RowMoves m, from;
+    stream_rows(dst, m);
+    stream_rows(src, from);
+    for (int k = 0; k < m.n; k++) m.src[k] = from.src[k];
+    return rows_move(m, d_index, dst->n, 0, src->n, st);
 }
 
 int32_t htm_is_fleet(const htm_engine* e) { return e && e->fleet ? 1 : 0; }

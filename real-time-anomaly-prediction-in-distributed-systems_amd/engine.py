@@ -225,6 +225,29 @@ class HTMEngine:
         """Copy stream `src` into every stream (config-2 setup)."""
         check(self._L.htm_replicate_stream(self.h, int(src), self._stream()))
 
+    def reorder_streams(self, parent):
+        """Fleets: stream g * beams + w goes on as stream g * beams + parent[g, w]
+        would have (parent: int32 device tensor [n_streams / beams, beams], beams
+        <= 64; a parent outside 0..beams-1 counts as w).  Every per-stream state
+        and output moves, in place; counters follow the state."""
+        if not isinstance(parent, torch.Tensor) or parent.dtype != torch.int32 or parent.dim() != 2 or \
+                parent.device != torch.device("cuda", self.device) or parent.numel() != self.n_streams:
+            raise ValueError(f"parent must be int32 [n_streams / beams, beams] on cuda:{self.device}")
+        p = parent.contiguous()
+        with torch.cuda.device(self.device):
+            check(self._L.htm_reorder_streams(self.h, ctypes.c_void_p(p.data_ptr()), int(p.shape[1]), self._stream()))
+
+    def copy_streams(self, src: "HTMEngine", index):
+        """Fleets of one model: stream s of this engine goes on as stream
+        index[s] of `src` (int32 device tensor [n_streams]; an index outside
+        src leaves s as it is) -- the fork of a fleet's streams into beams."""
+        if not isinstance(index, torch.Tensor) or index.dtype != torch.int32 or \
+                index.device != torch.device("cuda", self.device) or index.shape != (self.n_streams,):
+            raise ValueError(f"index must be int32 [{self.n_streams}] on cuda:{self.device}")
+        i = index.contiguous()
+        with torch.cuda.device(self.device):
+            check(self._L.htm_copy_streams(self.h, src.h, ctypes.c_void_p(i.data_ptr()), self._stream()))
+
     def device_bytes(self) -> int:
         return self._L.htm_device_bytes(self.h)
 

@@ -10,6 +10,8 @@
   TM learning switched off on the first test record while the SP keeps
   learning (NetworkModel.py:40-44), and 1 + 7 network steps per test record
   fed the same value (ModelTesting.py:66-72).
+* `model_forecast` -- a look-ahead that feeds its own predictions instead:
+  beams of bucket sequences per stream over the fleets of one model.
 """
 from __future__ import annotations
 
@@ -198,3 +200,91 @@ def model_testing(engine, cpu, violations, means, threshold=ANOMALY_SCORE, looka
         windows[r0:r0 + m] = sc.reshape(m, w, n).cpu().numpy()
         engine.status()  # raise on pool / queue overflow (NuPIC's NTA_THROW)
     return windows, slo.stats()
+
+
+def model_forecast(fleet, beam_fleet, readout, cpu, horizon=LOOKAHEAD, bucket_values=None, source="tm_output"):
+    """The next `horizon` values of every stream after each record.
+
+    The reference steps its network seven more times per record with the
+    record's own value (ModelTesting.py:66-72) and reads the classifier's seven
+    heads apart (NetworkUtils.py:166-184).  Here the network is fed what it
+    predicts: after a record's step every stream forks into `beams` copies;
+    each look-ahead step scores all (beam, bucket) continuations with the
+    one-step read-out, keeps the best `beams`, lets their states go on from
+    their parents' and feeds each its bucket's value.
+
+    fleet: HTMEngine.fleet of G streams; beam_fleet: one of G * beams streams
+    (beams <= 64) of the same model; readout: a Readout4 with one head, one
+    matrix or one a stream; cpu: [records] or [records, G].  bucket_values:
+    float64 [n_outputs], the value fed for each bucket (default: the scalar
+    encoder's bucket centres).  source: "tm_output" (cells) or
+    "col_confidence" (columns), what the read-out reads.
+
+    Returns dict(values float64 [records, horizon, G], the best beam's; logp
+    float32 [records, G], its log-probability; scores float32 [records, G], the
+    records' anomaly scores), on the host.  Streams whose read-out leaves no
+    bucket forecast NaN."""
+    import torch
+    from .beam import beam_reorder, beam_select
+    g = fleet.n_streams
+    if not fleet.is_fleet or not beam_fleet.is_fleet or beam_fleet.n_streams % g or beam_fleet is fleet:
+        raise ValueError("model_forecast needs two fleets of one model, of G and of G * beams streams")
+    if beam_fleet.n_streams // g > 64:
+        raise ValueError("at most 64 beams (got %d)" % (beam_fleet.n_streams // g))
+    if fleet.n_fields != 1:
+        raise ValueError("model_forecast follows one encoder field (got %d)" % fleet.n_fields)
+    beams, horizon = beam_fleet.n_streams // g, int(horizon)
+    if horizon < 1:
+        raise ValueError("horizon must be >= 1")
+    if readout.n_heads != 1 or readout.n_models not in (1, g):
+        raise ValueError("the read-out must have one head and one matrix, or one for each of the %d streams" % g)
+    if source not in ("tm_output", "col_confidence"):
+        raise ValueError("source must be 'tm_output' or 'col_confidence'")
+    dev = f"cuda:{fleet.device}"
+    c = fleet.config
+    if bucket_values is None:
+        if c.enc_type != _lib.ENC_SCALAR or readout.n_outputs > c.enc_n - c.enc_w + 1:
+            raise ValueError("give bucket_values: the read-out's outputs are not the scalar encoder's buckets")
+        lo, hi = (c.field_minval[0], c.field_maxval[0]) if c.field_maxval[0] > c.field_minval[0] else (c.enc_minval, c.enc_maxval)
+        bucket_values = lo + np.arange(readout.n_outputs) * ((hi - lo) / (c.enc_n - c.enc_w))
+    table = torch.as_tensor(bucket_values, dtype=torch.float64, device=dev).reshape(-1)
+    if table.numel() != readout.n_outputs:
+        raise ValueError("bucket_values needs one value per output (%d)" % readout.n_outputs)
+    table = torch.cat((table, table.new_full((1,), float("nan"))))  # [-1]: no bucket, a missing value
+    v = np.asarray(cpu, np.float64)
+    v = v[:, None] if v.ndim < 2 else v
+    v = torch.tensor(np.ascontiguousarray(np.broadcast_to(v, (v.shape[0], g))), device=dev)
+    n = v.shape[0]
+    live = None
+    if readout.live is not None:
+        live = readout.live if readout.n_models == g else readout.live.expand(g)
+    fork = torch.arange(g, dtype=torch.int32, device=dev).repeat_interleave(beams)
+    start = torch.zeros((g, 1), dtype=torch.float32, device=dev)
+    values = torch.empty((n, horizon, g), dtype=torch.float64, device=dev)
+    logp = torch.empty((n, g), dtype=torch.float32, device=dev)
+    scores = torch.empty((n, g), dtype=torch.float32, device=dev)
+    path = torch.empty((g, beams, horizon), dtype=torch.int32, device=dev)
+
+    def answer(eng, k):
+        x = eng.get_output(source)
+        y = readout.logits(x) if source == "tm_output" else readout.matvec(x)
+        return y.view(g, k, readout.n_outputs)
+
+    for t in range(n):
+        fleet.step(v[t], out=scores[t])
+        total, _, bucket = beam_select(answer(fleet, 1), start, beams, live=live)
+        path[:, :, 0] = bucket
+        for h in range(1, horizon):
+            if h == 1:
+                beam_fleet.copy_streams(fleet, fork)
+            beam_fleet.step(table[bucket.reshape(-1).long()])
+            total, parent, bucket = beam_select(answer(beam_fleet, beams), total, beams, live=live)
+            beam_reorder([path], parent)
+            path[:, :, h] = bucket
+            if h + 1 < horizon:
+                beam_fleet.reorder_streams(parent)
+        values[t] = table[path[:, 0].long()].t()
+        logp[t] = total[:, 0]
+    fleet.status()  # raise on pool / queue overflow (NuPIC's NTA_THROW)
+    beam_fleet.status()
+    return dict(values=values.cpu().numpy(), logp=logp.cpu().numpy(), scores=scores.cpu().numpy())
