@@ -12,6 +12,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+#include <type_traits>
+
 #include "htm_dev.h"
 #include "q4_dev.h"
 
@@ -149,74 +152,80 @@ struct Q4Acc {
 
 // The workgroup's threads are slots x blocks: thread (slot, block) has summed
 // its share of the inputs for one block's 32 outputs.  Sums over the slots, in
-// a fixed order, through LDS (16 of the 32 at a time); put(output, y) is called
-// once for each of the workgroup's nblk * 32 outputs.
-template <int NT, typename PUT>
-__device__ __forceinline__ void q4_join(Q4Acc& a, int nblk, int slots, float (*sm)[NT + 1], PUT put) {
-    const int nout = nblk * 16;
-    const int parts = nout < NT ? NT / nout : 1;
+// a fixed order, through LDS (16 of the 32 at a time, rows of nt + 1 floats);
+// put(output, y) is called once for each of the workgroup's nblk * 32 outputs.
+template <typename PUT>
+__device__ __forceinline__ void q4_join(Q4Acc& a, int nblk, int slots, float* sm, PUT put) {
+    const int nt = blockDim.x, nout = nblk * 16;
+    const int parts = nout < nt ? nt / nout : 1;
     const float off = 8.0f * a.s;
 #pragma unroll
     for (int half = 0; half < 2; half++) {
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 16; j++) sm[j][threadIdx.x] = a.v[half * 16 + j] - off;
+        for (int j = 0; j < 16; j++) sm[j * (nt + 1) + threadIdx.x] = a.v[half * 16 + j] - off;
         __syncthreads();
         if (parts == 1) {
-            for (int o = threadIdx.x; o < nout; o += NT) {
+            for (int o = threadIdx.x; o < nout; o += nt) {
+                const float* p = sm + (o & 15) * (nt + 1) + (o >> 4);
                 float y = 0.0f;
-                for (int s = 0; s < slots; s++) y += sm[o & 15][s * nblk + (o >> 4)];
+                for (int s = 0; s < slots; s++) y += p[s * nblk];
                 put((o >> 4) * Q4_BLK + half * 16 + (o & 15), y);
             }
         } else {  // few outputs: several threads each take a run of slots, then one adds up theirs
             const int part = threadIdx.x / nout, o = threadIdx.x - part * nout;
             const int each = (slots + parts - 1) / parts;
+            const float* p = sm + (o & 15) * (nt + 1) + (o >> 4);
             float y = 0.0f;
             if (part < parts)
-                for (int s = part * each; s < min(slots, part * each + each); s++) y += sm[o & 15][s * nblk + (o >> 4)];
+                for (int s = part * each; s < min(slots, part * each + each); s++) y += p[s * nblk];
             __syncthreads();
-            float* flat = &sm[0][0];
-            if (part < parts) flat[threadIdx.x] = y;
+            if (part < parts) sm[threadIdx.x] = y;
             __syncthreads();
             if (threadIdx.x < (uint32_t)nout) {
                 y = 0.0f;
-                for (int p = 0; p < parts; p++) y += flat[p * nout + o];
+                for (int k = 0; k < parts; k++) y += sm[k * nout + o];
                 put((o >> 4) * Q4_BLK + half * 16 + (o & 15), y);
             }
         }
     }
 }
 
-#define Q4_LIST 2048  // active inputs listed at a time
+#define Q4_LIST 2048   // active inputs listed at a time
+#define Q4_WORDS 8     // pattern words of a thread (65,536 inputs by 256 threads)
 
-// Word bitmaps.  One workgroup per (row, head, chunk of the head's blocks): the
-// active inputs are listed in LDS in ascending order, and each slot of threads
-// reads the records of every slots-th run of four, all blocks of the chunk side
-// by side.  SOFTMAX: the chunk is the whole head, whose probabilities are
-// written instead.
-template <int NT, bool SOFTMAX>
-__global__ void __launch_bounds__(NT) q4_rows_kernel(Q4Dims d, const uint8_t* __restrict__ rec,
-                                                     const uint32_t* __restrict__ pat, int64_t ps, int per_model,
-                                                     int row0, int chunks, int cblk, const int32_t* __restrict__ live,
-                                                     float* __restrict__ out) {
-    __shared__ float sm[16][NT + 1];
-    __shared__ __attribute__((aligned(8))) uint16_t list[Q4_LIST];
-    __shared__ uint32_t wsum[NT / 64];
-    __shared__ float y_sh[SOFTMAX ? Q4_MAX_SOFTMAX : 1];
-    const int row = row0 + blockIdx.y;
-    const int h = blockIdx.x / chunks, b0 = (blockIdx.x - h * chunks) * cblk;
-    const int nblk = min(cblk, d.nblk - b0);
-    const int slots = NT / nblk;
-    const int slot = threadIdx.x / nblk, b = threadIdx.x - slot * nblk;
+// Word bitmaps.  One workgroup per (row, run of cblk blocks of the record, which
+// may span heads).  The active inputs are listed in LDS in ascending order:
+// the words that are not empty are compacted first and then listed by two
+// threads each, since a bursting column sets a word's bits together.  Each slot takes
+// an even share of the list, its threads the run's blocks side by side, so that
+// a record is read in one piece.  SOFTMAX: the run is whole heads, whose
+// probabilities are written instead.
+template <bool SOFTMAX>
+__global__ void __launch_bounds__(1024) q4_rows_kernel(Q4Dims d, const uint8_t* __restrict__ rec,
+                                                       const uint32_t* __restrict__ pat, int64_t ps, int per_model,
+                                                       int row0, int cblk, const int32_t* __restrict__ live,
+                                                       float* __restrict__ out) {
+    __shared__ __attribute__((aligned(16))) uint32_t list[Q4_LIST];  // record offsets / 64
+    __shared__ uint32_t wsum[16];
+    extern __shared__ __attribute__((aligned(16))) float sm[];       // compacted words, then the join's rows
+    const int nt = blockDim.x, nwave = nt >> 6;
+    const int row = row0 + blockIdx.y, b0 = blockIdx.x * cblk;
+    const int nblk = min(cblk, d.nh * d.nblk - b0);
+    const int slots = nt / nblk;
+    const int slot = threadIdx.x / nblk, blk = b0 + threadIdx.x - slot * nblk;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t* p = pat + (int64_t)row * ps;
     const int words = d.ni / 32;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 
-    // the thread's words, their set bits' place among all
-    const int each = (words + NT - 1) / NT;
-    const int w0 = min(words, (int)threadIdx.x * each), w1 = min(words, w0 + each);
-    uint32_t mine = 0;
-    for (int w = w0; w < w1; w++) mine += __popc(p[w]);
+    // the thread's words: how many are not empty, and their bits
+    const int each = (words + nt - 1) / nt, w0 = threadIdx.x * each;
+    uint32_t x[Q4_WORDS], mine = 0;
+#pragma unroll
+    for (int k = 0; k < Q4_WORDS; k++) {
+        x[k] = k < each && w0 + k < words ? p[w0 + k] : 0u;
+        mine += __popc(x[k]) + (x[k] ? 1u << 18 : 0u);  // (at most 65,536 bits of 2,048 words)
+    }
     uint32_t at = mine;
     for (int k = 1; k < 64; k <<= 1) {
         const uint32_t o = __shfl_up(at, k);
@@ -224,86 +233,103 @@ __global__ void __launch_bounds__(NT) q4_rows_kernel(Q4Dims d, const uint8_t* __
     }
     if (lane == 63) wsum[wave] = at;
     __syncthreads();
-    uint32_t n = 0;
+    uint32_t all = 0;
     at -= mine;
-    for (int k = 0; k < NT / 64; k++) {
-        if (k < wave) at += wsum[k];
-        n += wsum[k];
+    for (int k = 0; k < nwave; k++) {
+        const uint32_t s = wsum[k];
+        if (k < wave) at += s;
+        all += s;
     }
+    const uint32_t n = all & 0x3FFFFu, full = all >> 18;
+    uint2* cw = reinterpret_cast<uint2*>(sm);
+#pragma unroll
+    for (int k = 0; k < Q4_WORDS; k++)
+        if (x[k]) {
+            cw[at >> 18] = make_uint2(x[k], ((uint32_t)(w0 + k) << 17) | (at & 0x3FFFFu));  // (a word begins below 65,536)
+            at += __popc(x[k]) + (1u << 18);
+        }
+    __syncthreads();
 
     Q4Acc acc;
     acc.clear();
-    const int blk = h * d.nblk + b0 + b;
+    const int h = blk / d.nblk;
     const uint8_t* base = rec + (int64_t)(row / per_model) * d.ni * d.pitch;
-    const uint32_t c_off = (uint32_t)blk * 16u;
-    const uint32_t s_off = d.scales + 2u * (uint32_t)(h * d.ngrp + (b0 + b) * Q4_BLK / d.group);
+    const uint8_t* cb = base + blk * 16;
+    const uint8_t* sb = base + d.scales + 2 * (h * d.ngrp + (blk - h * d.nblk) * Q4_BLK / d.group);
+    const uint32_t pitch64 = d.pitch / 64;
     for (uint32_t r0 = 0; r0 < n; r0 += Q4_LIST) {  // (a second round only beyond Q4_LIST active inputs)
         if (r0) __syncthreads();
-        uint32_t k = at;
-        for (int w = w0; w < w1; w++) {
-            uint32_t x = p[w];
-            while (x) {
-                const uint32_t q = k++ - r0;
-                if (q < Q4_LIST) list[q] = (uint16_t)(w * 32 + __ffs(x) - 1);
-                x &= x - 1;
-            }
+        for (uint32_t j = threadIdx.x >> 1; j < full; j += nt >> 1) {
+            const uint2 v = cw[j];
+            const uint32_t lo = v.x & 0xFFFFu;
+            uint32_t b = threadIdx.x & 1 ? v.x & 0xFFFF0000u : lo;
+            uint32_t q = (v.y & 0x1FFFFu) + (threadIdx.x & 1 ? __popc(lo) : 0) - r0;
+            const uint32_t first = (v.y >> 17) * 32u - 1u;
+            for (; b; b &= b - 1, q++)
+                if (q < Q4_LIST) list[q] = (first + __ffs(b)) * pitch64;
         }
         __syncthreads();
         const int m = (int)min(n - r0, (uint32_t)Q4_LIST);
-        if (slot < slots)
-            for (int i = slot * 4; i < m; i += slots * 4) {
-                const uint2 e = *reinterpret_cast<const uint2*>(list + i);
-                const uint32_t idx[4] = {e.x & 0xFFFFu, e.x >> 16, e.y & 0xFFFFu, e.y >> 16};
-                uint4 c[4];
-                float s[4];
+        if (slot < slots) {
+            // every slot's share, and one more for the first m % slots of them
+            const int share = m / slots, more = m - share * slots;
+            int i = slot * share + min(slot, more);
+            auto some = [&](auto count) {
+                constexpr int U = decltype(count)::value;
+                uint4 c[U];
+                uint32_t s[U];
 #pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    // (behind the list's end: the run's first record again, times zero)
-                    const uint8_t* r = base + (uint64_t)(i + u < m ? idx[u] : idx[0]) * d.pitch;
-                    c[u] = *reinterpret_cast<const uint4*>(r + c_off);
-                    const float v = bf16_up(*reinterpret_cast<const uint16_t*>(r + s_off));
-                    s[u] = i + u < m ? v : 0.0f;
+                for (int u = 0; u < U; u++) {
+                    const uint64_t r = (uint64_t)list[i + u] << 6;
+                    c[u] = *reinterpret_cast<const uint4*>(cb + r);
+                    s[u] = *reinterpret_cast<const uint16_t*>(sb + r);
                 }
+                __builtin_amdgcn_sched_barrier(0);  // (every load is under way before the first is waited for)
 #pragma unroll
-                for (int u = 0; u < 4; u++) acc.add(c[u], s[u]);
-            }
+                for (int u = 0; u < U; u++) acc.add(c[u], bf16_up(s[u]));
+                i += U;
+            };
+            for (int k = share; k >= 4; k -= 4) some(std::integral_constant<int, 4>());
+            if (share & 2) some(std::integral_constant<int, 2>());
+            if (share & 1) some(std::integral_constant<int, 1>());
+            if (slot < more) some(std::integral_constant<int, 1>());
+        }
     }
-    float* o = out + ((int64_t)row * d.nh + h) * d.no;
-    const int first = b0 * Q4_BLK;
+    float* o = out + (int64_t)row * d.nh * d.no;
     if (!SOFTMAX) {
-        q4_join<NT>(acc, nblk, slots, sm, [&](int k, float y) {
-            if (first + k < d.no) o[first + k] = y;
+        q4_join(acc, nblk, slots, sm, [&](int k, float y) {
+            const int b = b0 + (k >> 5), hh = b / d.nblk, j = (b - hh * d.nblk) * Q4_BLK + (k & 31);
+            if (j < d.no) o[hh * d.no + j] = y;
         });
         return;
     }
-    q4_join<NT>(acc, nblk, slots, sm, [&](int k, float y) { y_sh[k] = y; });
+    float* y_sh = sm + 16 * (nt + 1);
+    q4_join(acc, nblk, slots, sm, [&](int k, float y) { y_sh[k] = y; });
     __syncthreads();
+    // a wave per head
     int nl = d.no;
     if (live) nl = min(max(live[row / per_model], 0), d.no);
-    float* red = &sm[0][0];
-    float m = -INFINITY;
-    for (int k = threadIdx.x; k < nl; k += NT) m = fmaxf(m, y_sh[k]);
-    for (int k = 32; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
-    if (lane == 0) red[wave] = m;
-    __syncthreads();
-    for (int k = 0; k < NT / 64; k++) m = fmaxf(m, red[k]);
-    constexpr int PER = (Q4_MAX_SOFTMAX + NT - 1) / NT;
-    float e[PER], t = 0.0f;
+    const int stride = d.nblk * Q4_BLK;
+    for (int hh = wave; hh < nblk / d.nblk; hh += nwave) {
+        const float* y = y_sh + hh * stride;
+        float* q = o + (b0 / d.nblk + hh) * d.no;
+        float m = -INFINITY, t = 0.0f, v[Q4_MAX_SOFTMAX / 64];
 #pragma unroll
-    for (int j = 0; j < PER; j++) {
-        const int k = threadIdx.x + j * NT;
-        e[j] = k < nl ? expf(y_sh[k] - m) : 0.0f;
-        t += e[j];
-    }
-    for (int k = 32; k; k >>= 1) t += __shfl_xor(t, k);
-    if (lane == 0) red[64 + wave] = t;
-    __syncthreads();
-    t = 0.0f;
-    for (int k = 0; k < NT / 64; k++) t += red[64 + k];
+        for (int j = 0; j < Q4_MAX_SOFTMAX / 64; j++) {
+            const int k = j * 64 + lane;
+            v[j] = k < nl ? y[k] : -INFINITY;
+            m = fmaxf(m, v[j]);
+        }
+        for (int k = 32; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
 #pragma unroll
-    for (int j = 0; j < PER; j++) {
-        const int k = threadIdx.x + j * NT;
-        if (k < d.no) o[k] = k < nl ? e[j] / t : 0.0f;
+        for (int j = 0; j < Q4_MAX_SOFTMAX / 64; j++) {
+            v[j] = j * 64 + lane < nl ? expf(v[j] - m) : 0.0f;
+            t += v[j];
+        }
+        for (int k = 32; k; k >>= 1) t += __shfl_xor(t, k);
+#pragma unroll
+        for (int j = 0; j < Q4_MAX_SOFTMAX / 64; j++)
+            if (j * 64 + lane < d.no) q[j * 64 + lane] = j * 64 + lane < nl ? v[j] / t : 0.0f;
     }
 }
 
@@ -375,28 +401,51 @@ static int q4_bitmap(const htm_q4_shape* s, const void* rec, const uint32_t* pat
 
 #define Q4_GRID_Y 65535  // rows of one launch
 
-// Chunks of a head and the workgroup's width.  Many rows: whole heads (up to 32
-// blocks) by 256 threads.  Few workgroups: 1,024 threads each, and logits in
-// chunks down to one block until the chip's 256 CUs have one each, since then a
-// row's time is its longest chain of record reads.
+// More than 64 KiB of dynamic LDS: allowed once per kernel and device.
+static int q4_raise_lds(const void* kernel, size_t lds, std::atomic<uint64_t>& raised) {
+    if (lds <= 65536) return HTM_OK;
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return htm_fail(HTM_E_HIP, "q4: no current device");
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev < 64 && (raised.load() & bit)) return HTM_OK;
+    if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 150 * 1024) != hipSuccess)
+        return htm_fail(HTM_E_HIP, "q4: cannot raise the dynamic LDS limit to %zu B", lds);
+    if (dev < 64) raised.fetch_or(bit);
+    return HTM_OK;
+}
+
+// How a row's blocks are shared out.  Many rows: a workgroup takes whole records
+// (as many blocks as 512 threads hold; whole heads for a softmax), with the
+// width of 192 to 512 threads that leaves the fewest idle.  Few workgroups:
+// 1,024 threads each, and logits in runs down to one block until the chip's 256
+// CUs have one each, since then a row's time is its longest chain of reads.
 template <bool SOFTMAX>
-static void q4_rows_launch(const Q4Dims& d, const void* rec, const uint32_t* pat, int64_t ps, int32_t n_rows, int per,
-                           const int32_t* live, float* out, hipStream_t st) {
-    int chunks = (d.nblk + 31) / 32;
-    const bool wide = (int64_t)n_rows * d.nh * chunks < 512;
-    if (wide && !SOFTMAX)
-        while (chunks < d.nblk && (int64_t)n_rows * d.nh * chunks < 256) chunks++;
-    const int cblk = (d.nblk + chunks - 1) / chunks;
-    chunks = (d.nblk + cblk - 1) / cblk;
-    for (int32_t r0 = 0; r0 < n_rows; r0 += Q4_GRID_Y) {
-        const dim3 grid(d.nh * chunks, n_rows - r0 < Q4_GRID_Y ? n_rows - r0 : Q4_GRID_Y);
-        if (wide)
-            hipLaunchKernelGGL((q4_rows_kernel<1024, SOFTMAX>), grid, dim3(1024), 0, st, d, (const uint8_t*)rec, pat, ps,
-                               per, r0, chunks, cblk, live, out);
-        else
-            hipLaunchKernelGGL((q4_rows_kernel<256, SOFTMAX>), grid, dim3(256), 0, st, d, (const uint8_t*)rec, pat, ps,
-                               per, r0, chunks, cblk, live, out);
+static int q4_rows_launch(const Q4Dims& d, const void* rec, const uint32_t* pat, int64_t ps, int32_t n_rows, int per,
+                          const int32_t* live, float* out, hipStream_t st) {
+    const int total = d.nh * d.nblk, unit = SOFTMAX ? d.nblk : 1;
+    int chunks = (total + 511) / 512;
+    if (SOFTMAX) chunks = (d.nh + 512 / d.nblk - 1) / (512 / d.nblk);
+    const bool wide = (int64_t)n_rows * (SOFTMAX ? d.nh : chunks) < 512;
+    if (wide)
+        while (chunks < total / unit && (int64_t)n_rows * chunks < 256) chunks++;
+    const int cblk = ((total / unit + chunks - 1) / chunks) * unit;
+    chunks = (total + cblk - 1) / cblk;
+    int nt = 1024;
+    if (!wide) {
+        int best = 0;
+        for (int t = 256; t <= 512; t += 64) {
+            const int used = t / cblk * cblk * 1024 / t;
+            if (used > best + 20) best = used, nt = t;
+        }
     }
+    const size_t lds = (16 * (size_t)(nt + 1) + (SOFTMAX ? (size_t)cblk * Q4_BLK : 0)) * sizeof(float);
+    const auto kernel = q4_rows_kernel<SOFTMAX>;
+    static std::atomic<uint64_t> raised{0};  // devices whose limit of dynamic LDS is raised
+    if (int r = q4_raise_lds((const void*)kernel, lds, raised)) return r;
+    for (int32_t r0 = 0; r0 < n_rows; r0 += Q4_GRID_Y)
+        hipLaunchKernelGGL(kernel, dim3(chunks, n_rows - r0 < Q4_GRID_Y ? n_rows - r0 : Q4_GRID_Y), dim3(nt), lds, st, d,
+                           (const uint8_t*)rec, pat, ps, per, r0, cblk, live, out);
+    return hipGetLastError() == hipSuccess ? HTM_OK : htm_fail(HTM_E_HIP, "q4 rows launch failed");
 }
 
 extern "C" {
@@ -407,8 +456,7 @@ int htm_q4_logits(const htm_q4_shape* s, const void* rec, const uint32_t* pat, i
     int per;
     if (int r = q4_bitmap(s, rec, pat, ps, n_rows, out, __func__, &d, &per)) return r;
     if (!n_rows) return HTM_OK;
-    q4_rows_launch<false>(d, rec, pat, ps, n_rows, per, nullptr, out, (hipStream_t)stream);
-    return hipGetLastError() == hipSuccess ? HTM_OK : htm_fail(HTM_E_HIP, "q4 logits launch failed");
+    return q4_rows_launch<false>(d, rec, pat, ps, n_rows, per, nullptr, out, (hipStream_t)stream);
 }
 
 int htm_q4_probabilities(const htm_q4_shape* s, const void* rec, const uint32_t* pat, int64_t ps, const int32_t* live,
@@ -419,8 +467,7 @@ int htm_q4_probabilities(const htm_q4_shape* s, const void* rec, const uint32_t*
     if (d.no > Q4_MAX_SOFTMAX)
         return htm_fail(HTM_E_INVALID, "%s: at most %d outputs a head", __func__, Q4_MAX_SOFTMAX);
     if (!n_rows) return HTM_OK;
-    q4_rows_launch<true>(d, rec, pat, ps, n_rows, per, live, out, (hipStream_t)stream);
-    return hipGetLastError() == hipSuccess ? HTM_OK : htm_fail(HTM_E_HIP, "q4 probabilities launch failed");
+    return q4_rows_launch<true>(d, rec, pat, ps, n_rows, per, live, out, (hipStream_t)stream);
 }
 
 size_t htm_q4_work_bytes(const htm_q4_shape* s, int32_t n_rows) {
