@@ -459,7 +459,7 @@ int htm_cls_import_state(htm_classifier* cls, int32_t region, int32_t stream_beg
  * Records: uint8 [n_models][n_inputs][htm_q4_record_bytes], one input's weights:
  * per head the codes of its outputs (padded to a multiple of 32; the lower half
  * of a byte first), then per head ceil(padded / group) scales; padding is
- * ignored.  Base address and d_x / d_pattern / d_out as the element type asks,
+ * ignored; scales are finite and at most 2^100.  Base address and d_x / d_pattern / d_out as the element type asks,
  * records 16-byte aligned. */
 typedef struct {
     int32_t n_models;
@@ -478,7 +478,7 @@ size_t htm_q4_record_bytes(const htm_q4_shape* shape);
  * i * input_stride + h * head_stride + o) into d_records: scale = bfloat16(max|w| of
  * the group / 7), code = 8 + w / scale rounded to nearest even, within 1..15; a zero
  * stays exactly zero.  *d_bad (DEVICE int32, zeroed by the caller) is set to 1 if a
- * weight is infinite or NaN (its code is then meaningless). */
+ * weight is infinite or NaN, or above 7 * 2^100 (its code is then meaningless). */
 int htm_q4_quantise(const htm_q4_shape* shape, const void* d_weights, int32_t dtype, int64_t model_stride,
                     int64_t input_stride, int64_t head_stride, void* d_records, int32_t* d_bad, void* stream);
 /* The same from a classifier's streams [stream_begin, stream_begin + n_models) and

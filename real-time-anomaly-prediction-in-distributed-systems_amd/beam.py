@@ -12,7 +12,7 @@ import ctypes
 
 from . import _lib
 from ._lib import check
-from .readout import _stream, dtype_code
+from .readout import _On, dtype_code
 
 MAX_BEAMS = 64
 MAX_BUFFERS = 32
@@ -56,7 +56,7 @@ def beam_select(logits, scores, beams: int, live=None):
         gs, bs, _ = logits.stride()
     scores = scores.contiguous()
     live = live.contiguous() if live is not None else None
-    with torch.cuda.device(dev):
+    with _On(dev.index) as stream:
         o_score = torch.empty((groups, beams), dtype=torch.float32, device=dev)
         o_parent = torch.empty((groups, beams), dtype=torch.int32, device=dev)
         o_bucket = torch.empty((groups, beams), dtype=torch.int32, device=dev)
@@ -65,7 +65,7 @@ def beam_select(logits, scores, beams: int, live=None):
         check(L.htm_beam_select(logits.data_ptr(), code, gs, bs, scores.data_ptr(),
                                 live.data_ptr() if live is not None else None, groups, win, beams, v,
                                 o_score.data_ptr(), o_parent.data_ptr(), o_bucket.data_ptr(),
-                                work.data_ptr() if nb else None, nb, _stream(dev)))
+                                work.data_ptr() if nb else None, nb, stream))
     return o_score, o_parent, o_bucket
 
 
@@ -108,6 +108,6 @@ def beam_reorder(buffers, parent, out=None):
                 a.dtype != b.dtype or a.shape != b.shape or not a.is_contiguous() or not b.is_contiguous():
             raise ValueError("buffers and destinations must be contiguous, alike, and on %s" % dev)
         src_p[k], dst_p[k], size[k] = a.data_ptr(), b.data_ptr(), _row_bytes(a, groups, beams)
-    with torch.cuda.device(dev):
-        check(L.htm_beam_reorder(n, src_p, dst_p, size, parent.data_ptr(), groups, beams, _stream(dev)))
+    with _On(dev.index) as stream:
+        check(L.htm_beam_reorder(n, src_p, dst_p, size, parent.data_ptr(), groups, beams, stream))
     return dst

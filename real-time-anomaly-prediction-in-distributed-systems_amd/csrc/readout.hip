@@ -12,6 +12,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <atomic>
 #include <type_traits>
 
@@ -19,6 +20,7 @@
 #include "q4_dev.h"
 
 #define Q4_NT 256
+#define Q4_MAX_SCALE 1.2676506002282294e30  // 2^100: a scale times 2^24 stays finite (Q4Acc)
 
 int q4_dims(const htm_q4_shape* s, const char* who, Q4Dims* d) {
     if (!s) return htm_fail(HTM_E_INVALID, "%s: null shape", who);
@@ -73,8 +75,7 @@ __global__ void __launch_bounds__(Q4_NT) q4_quantise_kernel(Q4Dims d, const T* _
             odd |= !(a <= 1.7976931348623157e308);
             amax = fmax(amax, a);
         }
-        // (past the bfloat16 range on either side: no scale for the group's largest weight)
-        odd |= amax > 2.3e39;
+        odd |= amax > 7.0 * Q4_MAX_SCALE;
         const float s0 = (float)(amax / 7.0);
         const uint32_t sb = s0 >= 1.17549435e-38f && !odd ? bf16_round(s0) : 0u;
         const double s = (double)bf16_up(sb);
@@ -189,6 +190,27 @@ __device__ __forceinline__ void q4_join(Q4Acc& a, int nblk, int slots, float* sm
             }
         }
     }
+}
+
+// softmax of y[0..nl) to q[0..no), zero behind nl, by one wave (y == q is fine)
+__device__ __forceinline__ void q4_wave_softmax(const float* y, float* q, int nl, int no, int lane) {
+    float m = -INFINITY, t = 0.0f, v[Q4_MAX_SOFTMAX / 64];
+#pragma unroll
+    for (int j = 0; j < Q4_MAX_SOFTMAX / 64; j++) {
+        const int k = j * 64 + lane;
+        v[j] = k < nl ? y[k] : -INFINITY;
+        m = fmaxf(m, v[j]);
+    }
+    for (int k = 32; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
+#pragma unroll
+    for (int j = 0; j < Q4_MAX_SOFTMAX / 64; j++) {
+        v[j] = j * 64 + lane < nl ? expf(v[j] - m) : 0.0f;
+        t += v[j];
+    }
+    for (int k = 32; k; k >>= 1) t += __shfl_xor(t, k);
+#pragma unroll
+    for (int j = 0; j < Q4_MAX_SOFTMAX / 64; j++)
+        if (j * 64 + lane < no) q[j * 64 + lane] = j * 64 + lane < nl ? v[j] / t : 0.0f;
 }
 
 #define Q4_LIST 2048   // active inputs listed at a time
@@ -310,50 +332,202 @@ __global__ void __launch_bounds__(1024) q4_rows_kernel(Q4Dims d, const uint8_t* 
     int nl = d.no;
     if (live) nl = min(max(live[row / per_model], 0), d.no);
     const int stride = d.nblk * Q4_BLK;
-    for (int hh = wave; hh < nblk / d.nblk; hh += nwave) {
-        const float* y = y_sh + hh * stride;
-        float* q = o + (b0 / d.nblk + hh) * d.no;
-        float m = -INFINITY, t = 0.0f, v[Q4_MAX_SOFTMAX / 64];
+    for (int hh = wave; hh < nblk / d.nblk; hh += nwave)
+        q4_wave_softmax(y_sh + hh * stride, o + (b0 / d.nblk + hh) * d.no, nl, d.no, lane);
+}
+
+// The softmax alone, in place: a wave per (row, head).
+__global__ void __launch_bounds__(Q4_NT) q4_softmax_kernel(Q4Dims d, const int32_t* __restrict__ live, int per_model,
+                                                           int64_t total, float* __restrict__ y) {
+    const int64_t k = (int64_t)blockIdx.x * (Q4_NT / 64) + (threadIdx.x >> 6);
+    if (k >= total) return;
+    int nl = d.no;
+    if (live) nl = min(max(live[k / d.nh / per_model], 0), d.no);
+    q4_wave_softmax(y + k * d.no, y + k * d.no, nl, d.no, threadIdx.x & 63);
+}
+
+// Vectors of numbers.  One workgroup per (NX rows of one matrix, run of cb
+// half blocks, range of inputs): the inputs of a tile that are not zero in
+// every row are listed in LDS with the rows' numbers, the slots share the list
+// evenly, and a thread keeps its half block's 16 outputs of all NX rows, so that
+// a weight is read and unpacked once for all of them.  Here a code's bits get the
+// exponent under which they count ones (1024 + code, or 64 + code), and a packed
+// subtraction leaves code - 8, exactly: a weight takes part as the number it
+// stands for, with no correction behind the sum, at one instruction more per two
+// weights and rows.
+#define MV_NT 256
+#define MV_HB 16     // outputs of a half block
+
+template <int NX>
+struct MvAcc {
+    float v[NX][MV_HB];
+    __device__ __forceinline__ void add(uint2 c, float s, const float* x) {
+        const half2_t k0 = {(_Float16)1032.0f, (_Float16)1032.0f}, k1 = {(_Float16)72.0f, (_Float16)72.0f};
+        const uint32_t w[2] = {c.x, c.y};
+        const float m = NX == 1 ? s * x[0] : s;
 #pragma unroll
-        for (int j = 0; j < Q4_MAX_SOFTMAX / 64; j++) {
-            const int k = j * 64 + lane;
-            v[j] = k < nl ? y[k] : -INFINITY;
-            m = fmaxf(m, v[j]);
+        for (int k = 0; k < 2; k++) {
+            const uint32_t h = w[k] >> 8;
+            const half2_t q[4] = {as_half2((w[k] & 0x000F000Fu) | 0x64006400u) - k0,
+                                  as_half2((w[k] & 0x00F000F0u) | 0x54005400u) - k1,
+                                  as_half2((h & 0x000F000Fu) | 0x64006400u) - k0,
+                                  as_half2((h & 0x00F000F0u) | 0x54005400u) - k1};
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float n = (float)(j < 4 ? q[j & 3].x : q[j & 3].y);
+                if (NX == 1) {
+                    v[0][k * 8 + j] = __builtin_fmaf(n, m, v[0][k * 8 + j]);
+                } else {
+                    const float y = __builtin_fmaf(n, m, 0.0f);
+#pragma unroll
+                    for (int r = 0; r < NX; r++) v[r][k * 8 + j] = __builtin_fmaf(x[r], y, v[r][k * 8 + j]);
+                }
+            }
         }
-        for (int k = 32; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
+    }
+};
+
+template <typename T, int NX>
+__global__ void __launch_bounds__(MV_NT, NX == 8 ? 2 : NX == 4 ? 3 : 4)
+    q4_matvec_kernel(Q4Dims d, const uint8_t* __restrict__ rec, const T* __restrict__ x, int64_t xs, int per, int y0,
+                     int passes, int cb, int chunks, int range, float* __restrict__ out, int64_t split_stride) {
+    constexpr int KPT = 8 / NX, TILE = MV_NT * KPT;  // inputs of a thread and of a tile
+    __shared__ uint32_t list[TILE];
+    __shared__ __attribute__((aligned(16))) float xv[TILE][NX];
+    __shared__ uint32_t wsum[MV_NT / 64];
+    __shared__ float sm[MV_HB][MV_NT + 1];
+    const int chunk = blockIdx.x % chunks, split = blockIdx.x / chunks;
+    const int y = y0 + blockIdx.y, model = y / passes, q0 = (y - model * passes) * NX;
+    const int nx = min(NX, per - q0);
+    const int64_t row = (int64_t)model * per + q0;
+    const int halves = d.nh * d.nblk * 2, b0 = chunk * cb, nb = min(cb, halves - b0);
+    const int slots = MV_NT / nb, slot = threadIdx.x / nb, hb = b0 + threadIdx.x - slot * nb;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint8_t* base = rec + (int64_t)model * d.ni * d.pitch;
+    const int h = hb / (d.nblk * 2);
+    const uint8_t* cbase = base + hb * 8;
+    const uint8_t* sbase = base + d.scales + 2 * (h * d.ngrp + (hb - h * d.nblk * 2) * MV_HB / d.group);
+    const uint32_t pitch64 = d.pitch / 64;
+    const int k0 = split * range, k1 = min(d.ni, k0 + range);
+    MvAcc<NX> a;
 #pragma unroll
-        for (int j = 0; j < Q4_MAX_SOFTMAX / 64; j++) {
-            v[j] = j * 64 + lane < nl ? expf(v[j] - m) : 0.0f;
-            t += v[j];
+    for (int r = 0; r < NX; r++)
+#pragma unroll
+        for (int j = 0; j < MV_HB; j++) a.v[r][j] = 0.0f;
+    float mine[KPT][NX];  // inputs t0 + i * MV_NT + thread
+    auto fetch = [&](int t0) {
+#pragma unroll
+        for (int i = 0; i < KPT; i++) {
+            const int k = t0 + i * MV_NT + (int)threadIdx.x;
+#pragma unroll
+            for (int r = 0; r < NX; r++) mine[i][r] = k < k1 && r < nx ? x_up(x[(row + r) * xs + k]) : 0.0f;
         }
-        for (int k = 32; k; k >>= 1) t += __shfl_xor(t, k);
+    };
+    fetch(k0);
+    for (int t0 = k0; t0 < k1; t0 += TILE) {
+        uint64_t bal[KPT];
+        uint32_t cnt = 0;
 #pragma unroll
-        for (int j = 0; j < Q4_MAX_SOFTMAX / 64; j++)
-            if (j * 64 + lane < d.no) q[j * 64 + lane] = j * 64 + lane < nl ? v[j] / t : 0.0f;
+        for (int i = 0; i < KPT; i++) {
+            bool some = false;
+#pragma unroll
+            for (int r = 0; r < NX; r++) some |= mine[i][r] != 0.0f;
+            bal[i] = __ballot(some);
+            cnt += (uint32_t)__popcll(bal[i]);
+        }
+        if (lane == 0) wsum[wave] = cnt;
+        __syncthreads();
+        uint32_t at = 0, m = 0;
+#pragma unroll
+        for (int k = 0; k < MV_NT / 64; k++) {
+            if (k < wave) at += wsum[k];
+            m += wsum[k];
+        }
+#pragma unroll
+        for (int i = 0; i < KPT; i++) {
+            if ((bal[i] >> lane) & 1) {
+                const uint32_t q = at + (uint32_t)__popcll(bal[i] & ((1ull << lane) - 1ull));
+                list[q] = (uint32_t)(t0 + i * MV_NT + (int)threadIdx.x) * pitch64;
+#pragma unroll
+                for (int r = 0; r < NX; r++) xv[q][r] = mine[i][r];
+            }
+            at += (uint32_t)__popcll(bal[i]);
+        }
+        __syncthreads();
+        fetch(t0 + TILE);  // (the next tile's numbers meanwhile)
+        if (slot < slots) {
+            const int share = (int)m / slots, more = (int)m - share * slots;
+            int i = slot * share + min(slot, more);
+            auto step = [&](auto count) {
+                constexpr int U = decltype(count)::value;
+                uint2 c[U];
+                uint32_t s[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    const uint64_t r = (uint64_t)list[i + u] << 6;
+                    c[u] = *reinterpret_cast<const uint2*>(cbase + r);
+                    s[u] = *reinterpret_cast<const uint16_t*>(sbase + r);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    float xr[NX];
+#pragma unroll
+                    for (int r = 0; r < NX; r++) xr[r] = xv[i + u][r];
+                    a.add(c[u], bf16_up(s[u]), xr);
+                }
+                i += U;
+            };
+            int k = share;
+            for (; k >= 8; k -= 8) step(std::integral_constant<int, 8>());
+            if (k & 4) step(std::integral_constant<int, 4>());
+            if (k & 2) step(std::integral_constant<int, 2>());
+            if (k & 1) step(std::integral_constant<int, 1>());
+            if (slot < more) step(std::integral_constant<int, 1>());
+        }
+    }
+    float* o = out + split * split_stride + row * d.nh * d.no;
+    const int nout = nb * MV_HB;
+#pragma unroll
+    for (int r = 0; r < NX; r++) {
+        if (r >= nx) break;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < MV_HB; j++) sm[j][threadIdx.x] = a.v[r][j];
+        __syncthreads();
+        for (int k = threadIdx.x; k < nout; k += MV_NT) {
+            const float* p = &sm[k & 15][k >> 4];
+            float y = 0.0f;
+            for (int s = 0; s < slots; s++) y += p[s * nb];
+            const int b = b0 + (k >> 4), hh = b / (d.nblk * 2), j = (b - hh * d.nblk * 2) * MV_HB + (k & 15);
+            if (j < d.no) o[(int64_t)r * d.nh * d.no + hh * d.no + j] = y;
+        }
     }
 }
 
-// One thread per output: every input in turn.
-__device__ __forceinline__ float q4_weight(const uint8_t* __restrict__ r, const Q4Dims& d, int h, int o) {
-    const int at = h * d.nblk * Q4_BLK + o;
-    const int c = (r[at >> 1] >> ((at & 1) * 4)) & 15;
-    const uint32_t s = reinterpret_cast<const uint16_t*>(r + d.scales)[h * d.ngrp + o / d.group];
-    return bf16_up(s) * (float)(c - 8);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(Q4_NT) q4_matvec_kernel(Q4Dims d, const uint8_t* __restrict__ rec,
-                                                          const T* __restrict__ x, int64_t xs, int per_model,
-                                                          int row0, float* __restrict__ out) {
-    const int row = row0 + blockIdx.y;
-    const int k = blockIdx.x * Q4_NT + threadIdx.x;
-    if (k >= d.nh * d.no) return;
-    const int h = k / d.no, o = k - h * d.no;
-    const uint8_t* base = rec + (int64_t)(row / per_model) * d.ni * d.pitch;
-    const T* v = x + (int64_t)row * xs;
-    float acc = 0.0f;
-    for (int i = 0; i < d.ni; i++) acc = fmaf(x_up(v[i]), q4_weight(base + (int64_t)i * d.pitch, d, h, o), acc);
-    out[(int64_t)row * d.nh * d.no + k] = acc;
+// The ranges' sums added up: 64 outputs a workgroup, a quarter of the ranges a
+// wave, in a fixed order.
+__global__ void __launch_bounds__(256) q4_join_kernel(const float* __restrict__ part, int splits, int64_t n,
+                                                      float* __restrict__ out) {
+    __shared__ float sm[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t k = (int64_t)blockIdx.x * 64 + lane;
+    const int each = (splits + 3) / 4, s1 = min(splits, wave * each + each);
+    float y = 0.0f;
+    if (k < n) {
+        int s = wave * each;
+        for (; s + 8 <= s1; s += 8) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = part[(s + j) * n + k];
+#pragma unroll
+            for (int j = 0; j < 8; j++) y += v[j];
+        }
+        for (; s < s1; s++) y += part[s * n + k];
+    }
+    sm[wave][lane] = y;
+    __syncthreads();
+    if (wave == 0 && k < n) out[k] = (sm[0][lane] + sm[1][lane]) + (sm[2][lane] + sm[3][lane]);
 }
 
 // rows checked against the matrices; *per = rows that share one
@@ -401,6 +575,49 @@ static int q4_bitmap(const htm_q4_shape* s, const void* rec, const uint32_t* pat
 
 #define Q4_GRID_Y 65535  // rows of one launch
 
+// How a product is shared out: NX rows at a time, runs of half blocks and ranges
+// of inputs.
+struct MvPlan {
+    int nx, passes, cb, chunks, splits, range;
+};
+
+static MvPlan mv_plan(const Q4Dims& d, int per) {
+    MvPlan p;
+    p.nx = per >= 5 ? 8 : per >= 3 ? 4 : per;
+    p.passes = (per + p.nx - 1) / p.nx;
+    const int64_t y = (int64_t)d.nm * p.passes;
+    const int halves = d.nh * d.nblk * 2;
+    p.splits = 1;
+    if (d.ni <= 4096) {
+        p.chunks = (int)std::min<int64_t>(halves, std::max<int64_t>((halves + 31) / 32, 256 / y));
+    } else {
+        p.chunks = (halves + 31) / 32;
+        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / (p.chunks * y), d.ni / 256));
+    }
+    p.cb = (halves + p.chunks - 1) / p.chunks;
+    p.chunks = (halves + p.cb - 1) / p.cb;
+    p.range = (d.ni + p.splits - 1) / p.splits;
+    p.splits = (d.ni + p.range - 1) / p.range;
+    return p;
+}
+
+template <typename T>
+static void mv_launch(const MvPlan& p, const Q4Dims& d, const void* rec, const void* x, int64_t xs, int per, float* out,
+                      int64_t stride, hipStream_t st) {
+    const int64_t all = (int64_t)d.nm * p.passes;
+    for (int64_t y0 = 0; y0 < all; y0 += Q4_GRID_Y) {
+        const dim3 grid(p.chunks * p.splits, (uint32_t)std::min<int64_t>(all - y0, Q4_GRID_Y));
+        const auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, grid, dim3(MV_NT), 0, st, d, (const uint8_t*)rec, (const T*)x, xs, per, (int)y0, p.passes,
+                               p.cb, p.chunks, p.range, out, stride);
+        };
+        if (p.nx == 1) go(q4_matvec_kernel<T, 1>);
+        else if (p.nx == 2) go(q4_matvec_kernel<T, 2>);
+        else if (p.nx == 4) go(q4_matvec_kernel<T, 4>);
+        else go(q4_matvec_kernel<T, 8>);
+    }
+}
+
 // More than 64 KiB of dynamic LDS: allowed once per kernel and device.
 static int q4_raise_lds(const void* kernel, size_t lds, std::atomic<uint64_t>& raised) {
     if (lds <= 65536) return HTM_OK;
@@ -414,30 +631,30 @@ static int q4_raise_lds(const void* kernel, size_t lds, std::atomic<uint64_t>& r
     return HTM_OK;
 }
 
-// How a row's blocks are shared out.  Many rows: a workgroup takes whole records
-// (as many blocks as 512 threads hold; whole heads for a softmax), with the
-// width of 192 to 512 threads that leaves the fewest idle.  Few workgroups:
-// 1,024 threads each, and logits in runs down to one block until the chip's 256
-// CUs have one each, since then a row's time is its longest chain of reads.
+// How a row's blocks are shared out: runs of at most 64 blocks, or the whole
+// record (up to 512) where no two rows share a matrix and every record comes
+// from memory once; shorter runs until the chip's 256 CUs have a workgroup each.
+// Measured, us (runs x threads; 24,576 inputs, 480 outputs a head):
+//   4,096 rows of one matrix, 1 head: 1 x 256 103, 1 x 512 117, 2 x 256 113
+//   1,024 rows, 7 heads: 2 x 512 207, 1 x 1,024 239, 7 x 256 287
+//   256 rows of own matrices, 7 heads: 1 x 1,024 88, 2 x 512 96, 3 x 256 95
+//   64 rows, 7 heads: 4 x 512 28, 2 x 512 46, 1 x 1,024 74
+//   1 row, 7 heads: 105 x 256 8.9, 21 x 512 10.1, 105 x 1,024 12.6
 template <bool SOFTMAX>
 static int q4_rows_launch(const Q4Dims& d, const void* rec, const uint32_t* pat, int64_t ps, int32_t n_rows, int per,
                           const int32_t* live, float* out, hipStream_t st) {
-    const int total = d.nh * d.nblk, unit = SOFTMAX ? d.nblk : 1;
-    int chunks = (total + 511) / 512;
-    if (SOFTMAX) chunks = (d.nh + 512 / d.nblk - 1) / (512 / d.nblk);
-    const bool wide = (int64_t)n_rows * (SOFTMAX ? d.nh : chunks) < 512;
-    if (wide)
-        while (chunks < total / unit && (int64_t)n_rows * chunks < 256) chunks++;
-    const int cblk = ((total / unit + chunks - 1) / chunks) * unit;
-    chunks = (total + cblk - 1) / cblk;
-    int nt = 1024;
-    if (!wide) {
-        int best = 0;
-        for (int t = 256; t <= 512; t += 64) {
-            const int used = t / cblk * cblk * 1024 / t;
-            if (used > best + 20) best = used, nt = t;
-        }
+    const int total = d.nh * d.nblk;
+    int cblk;
+    if (SOFTMAX) {
+        cblk = d.nblk * std::max(1, std::min(d.nh, 64 / d.nblk));
+    } else {
+        int chunks = per == 1 && total <= 512 ? 1 : (total + 63) / 64;
+        chunks = std::min(total, std::max(chunks, 256 / n_rows));
+        cblk = (total + chunks - 1) / chunks;
     }
+    const int chunks = (total + cblk - 1) / cblk;
+    const bool few = (int64_t)n_rows * chunks <= 256;
+    const int nt = cblk > 64 ? 1024 : cblk > 24 || (few && cblk > 4) ? 512 : 256;
     const size_t lds = (16 * (size_t)(nt + 1) + (SOFTMAX ? (size_t)cblk * Q4_BLK : 0)) * sizeof(float);
     const auto kernel = q4_rows_kernel<SOFTMAX>;
     static std::atomic<uint64_t> raised{0};  // devices whose limit of dynamic LDS is raised
@@ -467,21 +684,29 @@ int htm_q4_probabilities(const htm_q4_shape* s, const void* rec, const uint32_t*
     if (d.no > Q4_MAX_SOFTMAX)
         return htm_fail(HTM_E_INVALID, "%s: at most %d outputs a head", __func__, Q4_MAX_SOFTMAX);
     if (!n_rows) return HTM_OK;
-    return q4_rows_launch<true>(d, rec, pat, ps, n_rows, per, live, out, (hipStream_t)stream);
+    hipStream_t st = (hipStream_t)stream;
+    if ((int64_t)n_rows * d.nh >= 256 || d.nblk == 1) return q4_rows_launch<true>(d, rec, pat, ps, n_rows, per, live, out, st);
+    // too few heads to fill the chip: the products in shorter runs, then the softmax (64 rows of 1,000 outputs: in
+    // one launch 30 us, the products 15.5)
+    if (int r = q4_rows_launch<false>(d, rec, pat, ps, n_rows, per, nullptr, out, st)) return r;
+    const int64_t k = (int64_t)n_rows * d.nh;
+    hipLaunchKernelGGL(q4_softmax_kernel, dim3((uint32_t)((k + Q4_NT / 64 - 1) / (Q4_NT / 64))), dim3(Q4_NT), 0, st, d, live,
+                       per, k, out);
+    return hipGetLastError() == hipSuccess ? HTM_OK : htm_fail(HTM_E_HIP, "q4 softmax launch failed");
 }
 
 size_t htm_q4_work_bytes(const htm_q4_shape* s, int32_t n_rows) {
     Q4Dims d;
-    (void)n_rows;
-    return q4_dims(s, __func__, &d) ? 0 : 0;
+    int per;
+    if (q4_dims(s, __func__, &d) || q4_rows(d, n_rows, __func__, &per) || !n_rows) return 0;
+    const MvPlan p = mv_plan(d, per);
+    return p.splits > 1 ? (size_t)p.splits * n_rows * d.nh * d.no * sizeof(float) : 0;
 }
 
 int htm_q4_matvec(const htm_q4_shape* s, const void* rec, const void* x, int32_t dtype, int64_t xs, int32_t n_rows,
                   float* out, void* work, size_t work_bytes, void* stream) {
     Q4Dims d;
     int per;
-    (void)work;
-    (void)work_bytes;
     if (int r = q4_dims(s, __func__, &d)) return r;
     if (int r = q4_rows(d, n_rows, __func__, &per)) return r;
     if (dtype != HTM_T_F32 && dtype != HTM_T_F16 && dtype != HTM_T_BF16)
@@ -489,19 +714,17 @@ int htm_q4_matvec(const htm_q4_shape* s, const void* rec, const void* x, int32_t
     if (!n_rows) return HTM_OK;
     if (int r = q4_aligned(rec, __func__)) return r;
     if (!x || !out || (n_rows > 1 && xs < d.ni)) return htm_fail(HTM_E_INVALID, "%s: invalid argument", __func__);
+    const MvPlan p = mv_plan(d, per);
+    const int64_t n = (int64_t)n_rows * d.nh * d.no;
+    if (p.splits > 1 && (!work || (uintptr_t)work % 4 || work_bytes < (size_t)(p.splits * n) * sizeof(float)))
+        return htm_fail(HTM_E_INVALID, "%s: needs htm_q4_work_bytes of scratch", __func__);
     hipStream_t st = (hipStream_t)stream;
-    for (int32_t r0 = 0; r0 < n_rows; r0 += Q4_GRID_Y) {
-        const dim3 grid((d.nh * d.no + Q4_NT - 1) / Q4_NT, n_rows - r0 < Q4_GRID_Y ? n_rows - r0 : Q4_GRID_Y);
-        if (dtype == HTM_T_F32)
-            hipLaunchKernelGGL(q4_matvec_kernel<float>, grid, dim3(Q4_NT), 0, st, d, (const uint8_t*)rec,
-                               (const float*)x, xs, per, r0, out);
-        else if (dtype == HTM_T_F16)
-            hipLaunchKernelGGL(q4_matvec_kernel<__half>, grid, dim3(Q4_NT), 0, st, d, (const uint8_t*)rec,
-                               (const __half*)x, xs, per, r0, out);
-        else
-            hipLaunchKernelGGL(q4_matvec_kernel<__hip_bfloat16>, grid, dim3(Q4_NT), 0, st, d, (const uint8_t*)rec,
-                               (const __hip_bfloat16*)x, xs, per, r0, out);
-    }
+    float* y = p.splits > 1 ? (float*)work : out;
+    if (dtype == HTM_T_F32) mv_launch<float>(p, d, rec, x, xs, per, y, n, st);
+    else if (dtype == HTM_T_F16) mv_launch<__half>(p, d, rec, x, xs, per, y, n, st);
+    else mv_launch<__hip_bfloat16>(p, d, rec, x, xs, per, y, n, st);
+    if (p.splits > 1)
+        hipLaunchKernelGGL(q4_join_kernel, dim3((uint32_t)((n + 63) / 64)), dim3(256), 0, st, y, p.splits, n, out);
     return hipGetLastError() == hipSuccess ? HTM_OK : htm_fail(HTM_E_HIP, "q4 matvec launch failed");
 }
 

@@ -32,9 +32,26 @@ def dtype_code(dtype) -> int:
     return _DTYPES.get(dtype, -1)
 
 
-def _stream(device):
-    import torch
-    return torch.cuda.current_stream(device).cuda_stream
+class _On:
+    """`with _On(index) as stream`: CUDA device `index` is current inside, `stream` its current stream's handle.
+    (torch.cuda.device and current_stream cost some 4 us a call, half of a small launch's host time.)"""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, index):
+        self.index = index
+
+    def __enter__(self):
+        import torch
+        self.before = torch._C._cuda_getDevice()
+        if self.before != self.index:
+            torch._C._cuda_setDevice(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            import torch
+            torch._C._cuda_setDevice(self.before)
 
 
 class Readout4:
@@ -66,6 +83,7 @@ class Readout4:
             raise ValueError("records must be 16-byte aligned")
         self.records = records
         self.device = records.device
+        self._index = records.device.index
         self._rec = records.data_ptr()
         self.live = None if live is None else self._live(live)
 
@@ -94,14 +112,14 @@ class Readout4:
             w = w.contiguous()
         nm, ni, nh, no = (int(k) for k in w.shape)
         per = cls.record_bytes(nm, ni, nh, no, group)
-        with torch.cuda.device(w.device):
+        with _On(w.device.index) as stream:
             rec = torch.zeros((nm, ni, per), dtype=torch.uint8, device=w.device)
             bad = torch.zeros(1, dtype=torch.int32, device=w.device)
             self = cls(rec, ni, nh, no, group, live)
             check(self._L.htm_q4_quantise(self._pshape, w.data_ptr(), dtype_code(w.dtype), w.stride(0), w.stride(1),
-                                          w.stride(2), self._rec, bad.data_ptr(), _stream(w.device)))
+                                          w.stride(2), self._rec, bad.data_ptr(), stream))
             if bad.item():
-                raise ValueError("weights must be finite (and within bfloat16's range)")
+                raise ValueError("weights must be finite (and at most 7 * 2**100)")
         return self
 
     @classmethod
@@ -121,13 +139,13 @@ class Readout4:
             raise ValueError("steps %s are not neighbours in the classifier's %s" % (steps, classifier.steps))
         dev = torch.device("cuda", classifier.device)
         per = cls.record_bytes(n, classifier.n_inputs, nh, classifier.n_buckets, group)
-        with torch.cuda.device(dev):
+        with _On(dev.index) as stream:
             rec = torch.zeros((n, classifier.n_inputs, per), dtype=torch.uint8, device=dev)
             live = torch.empty(n, dtype=torch.int32, device=dev)
             bad = torch.zeros(1, dtype=torch.int32, device=dev)
             self = cls(rec, classifier.n_inputs, nh, classifier.n_buckets, group, live)
             check(self._L.htm_cls_quantise(classifier.h, int(s0), y0, self._pshape, self._rec, live.data_ptr(),
-                                           bad.data_ptr(), _stream(dev)))
+                                           bad.data_ptr(), stream))
             if bad.item():
                 raise ValueError("the classifier's weights are not finite")
         return self
@@ -176,26 +194,22 @@ class Readout4:
         """y [rows, n_heads, n_outputs] float32 of word bitmaps [rows,
         n_inputs / 32] (the engine's "tm_output"): bit b of word w is input
         32 w + b.  A row without a set bit gives zeros."""
-        import torch
         p, n, stride = self._pattern(pattern)
         y = self._out(out, n)
-        with torch.cuda.device(self.device):
-            check(self._L.htm_q4_logits(self._pshape, self._rec, p.data_ptr(), stride, n, y.data_ptr(),
-                                        _stream(self.device)))
+        with _On(self._index) as stream:
+            check(self._L.htm_q4_logits(self._pshape, self._rec, p.data_ptr(), stride, n, y.data_ptr(), stream))
         return y
 
     def probabilities(self, pattern, live=None, out=None):
         """softmax of `logits` over each head's first `live` outputs (int32
         [n_models]; default: the read-out's own, or all of them), 0 above: the
         classifier region's "probabilities".  n_outputs <= 1024."""
-        import torch
         p, n, stride = self._pattern(pattern)
         lv = self.live if live is None else self._live(live)
         y = self._out(out, n)
-        with torch.cuda.device(self.device):
+        with _On(self._index) as stream:
             check(self._L.htm_q4_probabilities(self._pshape, self._rec, p.data_ptr(), stride,
-                                               lv.data_ptr() if lv is not None else None, n, y.data_ptr(),
-                                               _stream(self.device)))
+                                               lv.data_ptr() if lv is not None else None, n, y.data_ptr(), stream))
         return y
 
     def matvec(self, x, out=None):
@@ -207,10 +221,10 @@ class Readout4:
         v, n, stride = self._rows(x, self.n_inputs, "x")
         y = self._out(out, n)
         nb = self._L.htm_q4_work_bytes(self._pshape, n)
-        with torch.cuda.device(self.device):
+        with _On(self._index) as stream:
             work = torch.empty(nb, dtype=torch.uint8, device=self.device) if nb else None
             check(self._L.htm_q4_matvec(self._pshape, self._rec, v.data_ptr(), dtype_code(v.dtype), stride, n,
-                                        y.data_ptr(), work.data_ptr() if nb else None, nb, _stream(self.device)))
+                                        y.data_ptr(), work.data_ptr() if nb else None, nb, stream))
         return y
 
     def device_bytes(self) -> int:
