@@ -10,26 +10,138 @@
 #include "beam_dev.h"
 #include "htm_dev.h"
 
-#define BS_NT 256
 #define BS_MAX 64  // beams
 
 __device__ __forceinline__ float up(float v) { return v; }
 __device__ __forceinline__ float up(__half v) { return __half2float(v); }
 __device__ __forceinline__ float up(__hip_bfloat16 v) { return __bfloat162float(v); }
 
+// ------------------------------------------------------------------ selection
 // (score, place) as one unsigned key: larger is better, equal scores by the
-// lower place; 0: never taken
-__device__ __forceinline__ uint64_t cand_key(float s, uint32_t place) {
+// lower place; 0: never taken.  The upper word alone orders the scores.
+__device__ __forceinline__ uint32_t score_bits(float s) {
     s += 0.0f;  // -0 and 0 are the same score
     if (!(s > -INFINITY)) return 0;
     const uint32_t u = __float_as_uint(s);
-    const uint32_t o = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-    return ((uint64_t)o << 32) | (0xFFFFFFFFu - place);
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-__device__ __forceinline__ float key_score(uint64_t k) {
-    const uint32_t o = (uint32_t)(k >> 32);
+__device__ __forceinline__ float bits_score(uint32_t o) {
     return __uint_as_float((o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
+}
+
+__device__ __forceinline__ uint64_t make_key(uint32_t bits, uint32_t place) {
+    return bits ? ((uint64_t)bits << 32) | (0xFFFFFFFFu - place) : 0;
+}
+
+// 2^t for t <= 0, relative error below 2^-46: the Taylor series of exp to degree
+// 11 on |f ln 2| <= 0.347 (remainder 0.347^12 / 12! = 6e-15).  A rounding border
+// of a float32 score is then missed once in some 10^6 candidates by one step,
+// as any other order of the same float64 sum would miss it.
+__device__ __forceinline__ double exp2_neg(double t) {
+    const double n = rint(t), f = (t - n) * 0.69314718055994530942;
+    double p = 1.0 / 39916800.0;
+    p = fma(p, f, 1.0 / 3628800.0);
+    p = fma(p, f, 1.0 / 362880.0);
+    p = fma(p, f, 1.0 / 40320.0);
+    p = fma(p, f, 1.0 / 5040.0);
+    p = fma(p, f, 1.0 / 720.0);
+    p = fma(p, f, 1.0 / 120.0);
+    p = fma(p, f, 1.0 / 24.0);
+    p = fma(p, f, 1.0 / 6.0);
+    p = fma(p, f, 0.5);
+    p = fma(p, f, 1.0);
+    p = fma(p, f, 1.0);
+    return ldexp(p, (int)fmax(n, -2000.0));
+}
+
+// exp(x - m) of float32 numbers; x = -inf gives 0, a NaN or x - m = NaN gives NaN
+__device__ __forceinline__ double exp_diff(float x, float m) {
+    const double t = ((double)x - (double)m) * 1.4426950408889634074;
+    return t > -1100.0 ? exp2_neg(t) : (t == t ? 0.0 : t);
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+    for (int k = 32; k; k >>= 1) v = fmaxf(v, __shfl_xor(v, k));
+    return v;
+}
+
+__device__ __forceinline__ double wave_sum(double v) {
+    for (int k = 32; k; k >>= 1) v += __shfl_xor(v, k);
+    return v;
+}
+
+struct TopSh {
+    uint64_t floor;  // the want-th best of the threads' best
+    uint32_t count;  // candidates that reach it
+};
+
+// The best `want` (<= 64) of the candidates held in LDS: bits[0..n), places place0
+// + index, nt = blockDim.x threads, tops: room for want keys a wave, list: for
+// want * ceil(n / nt) keys.
+// Every thread's best candidate first; the want-th best of those is a floor that
+// at least `want` candidates reach (or all there are), and at most want threads
+// hold any that do, so a short list is left, whose members count those before
+// them.  put(rank, key) is called once for each candidate taken.  Every step is
+// a comparison of distinct keys: the result does not depend on the order in
+// which the list was filled.
+template <typename PUT>
+__device__ __forceinline__ void top_of(const uint32_t* bits, int n, uint32_t place0, int want, TopSh& sh, uint64_t* tops,
+                                       uint64_t* list, PUT put) {
+    const int nt = blockDim.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nwave = nt >> 6;
+    uint32_t best = 0, at = 0;
+    for (int i = threadIdx.x; i < n; i += nt) {
+        const uint32_t b = bits[i];
+        if (b > best) best = b, at = i;
+    }
+    const uint64_t mine = make_key(best, place0 + at);
+    if (want >= 64) {
+        tops[threadIdx.x] = mine;
+    } else {
+        uint32_t cur = best;
+        uint64_t won = 0;  // lane r: the wave's r-th best
+        for (int r = 0; r < want; r++) {
+            const uint32_t top = wave_max_u32(cur);
+            if (!top) break;
+            uint64_t eq = __ballot(cur == top);
+            if (eq & (eq - 1)) {  // equal scores: the lowest place of them
+                const uint32_t low = ~wave_max_u32(cur == top ? ~at : 0u);
+                eq = __ballot(cur == top && at == low);
+            }
+            const int src = __ffsll((unsigned long long)eq) - 1;
+            const uint32_t p = (uint32_t)__builtin_amdgcn_readlane((int)at, src);
+            if (lane == r) won = make_key(top, place0 + p);
+            if (lane == src) cur = 0;
+        }
+        if (lane < want) tops[wave * want + lane] = won;
+    }
+    if (threadIdx.x == 0) {
+        sh.floor = 1;
+        sh.count = 0;
+    }
+    __syncthreads();
+    const int held = nwave * min(want, 64);
+    if ((int)threadIdx.x < held) {
+        const uint64_t k = tops[threadIdx.x];
+        int before = 0;
+        for (int j = 0; j < held; j++) before += tops[j] > k ? 1 : 0;
+        if (k && before == want - 1) sh.floor = k;
+    }
+    __syncthreads();
+    const uint64_t floor = sh.floor;
+    if (mine >= floor)
+        for (int i = threadIdx.x; i < n; i += nt) {
+            const uint64_t k = make_key(bits[i], place0 + (uint32_t)i);
+            if (k >= floor) list[atomicAdd(&sh.count, 1u)] = k;
+        }
+    __syncthreads();
+    const int m = (int)sh.count;
+    for (int i = threadIdx.x; i < m; i += nt) {
+        const uint64_t k = list[i];
+        int before = 0;
+        for (int j = 0; j < m; j++) before += list[j] > k ? 1 : 0;
+        if (before < want) put(before, k);
+    }
 }
 
 struct SelArgs {
@@ -43,58 +155,221 @@ struct SelArgs {
     int32_t* o_bucket;
 };
 
-// One workgroup per group: every beam's log-sum-exp, then the best key below
-// the last one taken, n_beams times.
+__device__ __forceinline__ int live_of(const SelArgs& a, int64_t g) {
+    return a.live ? min(max(a.live[g], 0), a.v) : a.v;
+}
+
+__device__ __forceinline__ void put_key(const SelArgs& a, int64_t g, int rank, uint64_t k) {
+    const int64_t at = g * a.wout + rank;
+    const uint32_t place = 0xFFFFFFFFu - (uint32_t)k;
+    a.o_score[at] = bits_score((uint32_t)(k >> 32));
+    a.o_parent[at] = (int32_t)(place / (uint32_t)a.v);
+    a.o_bucket[at] = (int32_t)(place % (uint32_t)a.v);
+}
+
+__device__ __forceinline__ void put_rest(const SelArgs& a, int64_t g, int taken) {
+    for (int r = taken + (int)threadIdx.x; r < a.wout; r += blockDim.x) {
+        const int64_t at = g * a.wout + r;
+        a.o_score[at] = -INFINITY;
+        a.o_parent[at] = min(r, a.win - 1);
+        a.o_bucket[at] = -1;
+    }
+}
+
+// Few candidates (beams_in * n_outputs <= BS_ONE): one workgroup per group, the
+// logits read once into LDS.  parts waves share a beam.
+#define BS_ONE 8192
 template <typename T>
-__global__ void __launch_bounds__(BS_NT) beam_select_kernel(SelArgs a) {
-    __shared__ double base[BS_MAX];  // score - log(sum)
+__global__ void __launch_bounds__(1024) beam_select_kernel(SelArgs a, int parts) {
+    __shared__ TopSh sh;
+    __shared__ double sum[BS_MAX];  // [beam * parts + part]: parts > 1 only while beams * parts <= waves
     __shared__ float top[BS_MAX];
-    __shared__ uint64_t red[BS_NT / 64];
-    const int g = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const T* x = (const T*)a.x + (int64_t)g * a.gs;
-    int n = a.v;
-    if (a.live) n = min(max(a.live[g], 0), a.v);
-    for (int w = wave; w < a.win; w += BS_NT / 64) {
+    extern __shared__ __attribute__((aligned(16))) uint32_t cand[];  // [win * v] logits, then score bits; tops; list
+    const int64_t g = blockIdx.x;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nwave = blockDim.x >> 6;
+    const int n = live_of(a, g), rows = nwave / parts, part = wave % parts;
+    const T* x = (const T*)a.x + g * a.gs;
+    const int step = parts * 64;
+    for (int w = wave / parts; w < a.win; w += rows) {
         const T* p = x + (int64_t)w * a.bs;
+        uint32_t* c = cand + w * a.v;
         float m = -INFINITY;
-        for (int o = lane; o < n; o += 64) m = fmaxf(m, up(p[o]));
-        for (int k = 32; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
-        double s = 0.0;
-        for (int o = lane; o < n; o += 64) s += exp((double)up(p[o]) - (double)m);
-        for (int k = 32; k; k >>= 1) s += __shfl_xor(s, k);
-        // (no finite logit, an infinite one or a NaN: the sum is 0 or NaN, and no score of the beam is a number)
-        if (lane == 0) {
-            base[w] = (double)a.score[(int64_t)g * a.win + w] - log(s);
-            top[w] = m;
+        int o = part * 64 + lane;
+        for (; o + 7 * step < n; o += 8 * step) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = up(p[o + j * step]);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                c[o + j * step] = __float_as_uint(v[j]);
+                m = fmaxf(m, v[j]);
+            }
         }
+#pragma unroll 4
+        for (; o < n; o += step) {
+            const float v = up(p[o]);
+            c[o] = __float_as_uint(v);
+            m = fmaxf(m, v);
+        }
+        m = wave_max(m);
+        if (lane == 0) top[w * parts + part] = m;
     }
     __syncthreads();
+    for (int w = wave / parts; w < a.win; w += rows) {
+        float m = top[w * parts];
+        for (int k = 1; k < parts; k++) m = fmaxf(m, top[w * parts + k]);
+        const uint32_t* c = cand + w * a.v;
+        double s = 0.0;
+#pragma unroll 2
+        for (int o = part * 64 + lane; o < n; o += step) s += exp_diff(__uint_as_float(c[o]), m);
+        s = wave_sum(s);
+        if (lane == 0) sum[w * parts + part] = s;
+    }
+    __syncthreads();
+    for (int w = wave / parts; w < a.win; w += rows) {
+        float m = top[w * parts];
+        double s = sum[w * parts];
+        for (int k = 1; k < parts; k++) {
+            m = fmaxf(m, top[w * parts + k]);
+            s += sum[w * parts + k];
+        }
+        // (no finite logit, an infinite one or a NaN: the sum is 0 or NaN, and no score of the beam is a number)
+        const double base = (double)a.score[g * a.win + w] - log(s);
+        uint32_t* c = cand + w * a.v;
+        for (int o = part * 64 + lane; o < a.v; o += step)
+            c[o] = o < n ? score_bits((float)(((double)__uint_as_float(c[o]) - (double)m) + base)) : 0u;
+    }
+    __syncthreads();
+    const int all = a.win * a.v;
+    uint64_t* tops = reinterpret_cast<uint64_t*>(cand + ((all + 1) & ~1));
+    top_of(cand, all, 0, a.wout, sh, tops, tops + nwave * a.wout, [&](int r, uint64_t k) { put_key(a, g, r, k); });
+    __syncthreads();
+    put_rest(a, g, min((int)sh.count, a.wout));
+}
+
+// Many candidates: chunks of BS_CHUNK of a beam's outputs, three launches.
+#define BS_CHUNK 4096
+struct SelWork {
+    float* top;      // [groups * win * chunks] the chunks' largest logits
+    double* sum;     // ... and sums of exp(x - top)
+    uint64_t* keys;  // [groups * win * chunks * wout] the chunks' best
+    int32_t chunks;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) beam_sums_kernel(SelArgs a, SelWork k, int64_t row0) {
+    __shared__ float tm[4];
+    __shared__ double ts[4];
+    const int64_t row = row0 + blockIdx.y, g = row / a.win;
+    const int o0 = blockIdx.x * BS_CHUNK, n = min(live_of(a, g), o0 + BS_CHUNK);
+    const T* p = (const T*)a.x + g * a.gs + (row - g * a.win) * a.bs;
+    float v[BS_CHUNK / 256], m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < BS_CHUNK / 256; j++) {
+        const int o = o0 + j * 256 + threadIdx.x;
+        v[j] = o < n ? up(p[o]) : -INFINITY;
+        m = fmaxf(m, v[j]);
+    }
+    m = wave_max(m);
+    if ((threadIdx.x & 63) == 0) tm[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(tm[0], tm[1]), fmaxf(tm[2], tm[3]));
+    double s = 0.0;
+#pragma unroll
+    for (int j = 0; j < BS_CHUNK / 256; j++)
+        if (o0 + j * 256 + (int)threadIdx.x < n) s += m > -INFINITY ? exp_diff(v[j], m) : v[j] == v[j] ? 0.0 : (double)v[j];
+    s = wave_sum(s);
+    if ((threadIdx.x & 63) == 0) ts[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        k.top[row * k.chunks + blockIdx.x] = m;
+        k.sum[row * k.chunks + blockIdx.x] = (ts[0] + ts[1]) + (ts[2] + ts[3]);
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) beam_chunk_kernel(SelArgs a, SelWork k, int64_t row0) {
+    __shared__ TopSh sh;
+    __shared__ uint32_t cand[BS_CHUNK];
+    __shared__ uint64_t tops[BS_MAX * 4], list[BS_MAX * (BS_CHUNK / 256)];
+    __shared__ float tm[4];
+    __shared__ double ts[4];
+    const int64_t row = row0 + blockIdx.y, g = row / a.win;
+    const int o0 = blockIdx.x * BS_CHUNK, n = min(live_of(a, g), o0 + BS_CHUNK), w = (int)(row - g * a.win);
+    const T* p = (const T*)a.x + g * a.gs + w * a.bs;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    float v[BS_CHUNK / 256];
+#pragma unroll
+    for (int j = 0; j < BS_CHUNK / 256; j++) {
+        const int o = o0 + j * 256 + threadIdx.x;
+        v[j] = o < n ? up(p[o]) : -INFINITY;
+    }
+    // the beam's largest logit and sum from its chunks'
+    const float* top = k.top + row * k.chunks;
+    const double* sum = k.sum + row * k.chunks;
+    float m = -INFINITY;
+    for (int c = threadIdx.x; c < k.chunks; c += 256) m = fmaxf(m, top[c]);
+    m = wave_max(m);
+    if (lane == 0) tm[wave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(tm[0], tm[1]), fmaxf(tm[2], tm[3]));
+    double s = 0.0;
+    for (int c = threadIdx.x; c < k.chunks; c += 256)
+        if (top[c] > -INFINITY || sum[c] != 0.0) s += sum[c] * exp_diff(top[c], m);  // (a chunk without a live output adds nothing)
+    s = wave_sum(s);
+    if (lane == 0) ts[wave] = s;
+    __syncthreads();
+    s = (ts[0] + ts[1]) + (ts[2] + ts[3]);
+    const double base = (double)a.score[row] - log(s);
+#pragma unroll
+    for (int j = 0; j < BS_CHUNK / 256; j++) {
+        const int i = j * 256 + threadIdx.x;
+        cand[i] = o0 + i < n ? score_bits((float)(((double)v[j] - (double)m) + base)) : 0u;
+    }
+    __syncthreads();
+    uint64_t* keys = k.keys + (row * k.chunks + blockIdx.x) * a.wout;
+    top_of(cand, BS_CHUNK, (uint32_t)(w * (int64_t)a.v + o0), a.wout, sh, tops, list, [&](int r, uint64_t key) { keys[r] = key; });
+    __syncthreads();
+    for (int r = (int)sh.count + (int)threadIdx.x; r < a.wout; r += 256) keys[r] = 0;
+}
+
+// The chunks' best of one group: each thread its own of the keys, the best key
+// below the last one taken, wout times.
+__global__ void __launch_bounds__(1024) beam_merge_kernel(SelArgs a, SelWork k) {
+    __shared__ uint64_t red[16];
+    const int64_t g = blockIdx.x;
+    const int64_t n = (int64_t)a.win * k.chunks * a.wout;
+    const uint64_t* keys = k.keys + g * n;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nwave = blockDim.x >> 6;
+    constexpr int HELD = 8;  // keys of a thread in registers; any more are read again
+    uint64_t mine[HELD];
+#pragma unroll
+    for (int j = 0; j < HELD; j++) {
+        const int64_t i = (int64_t)j * blockDim.x + threadIdx.x;
+        mine[j] = i < n ? keys[i] : 0;
+    }
     uint64_t prev = ~0ull;
-    for (int j = 0; j < a.wout; j++) {
+    int r = 0;
+    for (; r < a.wout; r++) {
         uint64_t best = 0;
-        for (int w = 0; w < a.win; w++)
-            for (int o = threadIdx.x; o < n; o += BS_NT) {
-                const float s = (float)(((double)up(x[(int64_t)w * a.bs + o]) - (double)top[w]) + base[w]);
-                const uint64_t k = cand_key(s, (uint32_t)(w * a.v + o));
-                if (k < prev && k > best) best = k;
-            }
-        for (int k = 32; k; k >>= 1) {
-            const uint64_t other = __shfl_xor((unsigned long long)best, k);
-            best = other > best ? other : best;
-        }
-        if (lane == 0) red[wave] = best;
+#pragma unroll
+        for (int j = 0; j < HELD; j++)
+            if (mine[j] < prev && mine[j] > best) best = mine[j];
+        for (int64_t i = (int64_t)HELD * blockDim.x + threadIdx.x; i < n; i += blockDim.x)
+            if (keys[i] < prev && keys[i] > best) best = keys[i];
+        // the upper word's largest, then the lower word's among those
+        const uint32_t hi = wave_max_u32((uint32_t)(best >> 32));
+        const uint32_t lo = wave_max_u32((uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
+        if (lane == 0) red[wave] = ((uint64_t)hi << 32) | lo;
         __syncthreads();
-        for (int k = 0; k < BS_NT / 64; k++) best = red[k] > best ? red[k] : best;
+        best = 0;
+        for (int j = 0; j < nwave; j++) best = red[j] > best ? red[j] : best;
         __syncthreads();
-        if (threadIdx.x == 0) {
-            const int64_t at = (int64_t)g * a.wout + j;
-            const uint32_t place = 0xFFFFFFFFu - (uint32_t)best;
-            a.o_score[at] = best ? key_score(best) : -INFINITY;
-            a.o_parent[at] = best ? (int32_t)(place / (uint32_t)a.v) : min(j, a.win - 1);
-            a.o_bucket[at] = best ? (int32_t)(place % (uint32_t)a.v) : -1;
-        }
+        if (!(best >> 32)) break;
+        if (threadIdx.x == 0) put_key(a, g, r, best);
         prev = best;
     }
+    put_rest(a, g, r);
 }
 
 // ------------------------------------------------------------------- rows
@@ -172,16 +447,48 @@ int rows_move(const RowMoves& m, const int32_t* idx, int64_t n_rows, int32_t bea
 
 extern "C" {
 
-size_t htm_beam_work_bytes(int32_t n_groups, int32_t beams_in, int32_t n_beams, int32_t n_outputs) {
-    (void)n_groups; (void)beams_in; (void)n_beams; (void)n_outputs;
-    return 0;
+static int sel_chunks(int32_t v) { return (v + BS_CHUNK - 1) / BS_CHUNK; }
+
+size_t htm_beam_work_bytes(int32_t groups, int32_t win, int32_t wout, int32_t v) {
+    if (groups < 1 || win < 1 || win > BS_MAX || wout < 1 || wout > BS_MAX || v < 1 || (int64_t)win * v <= BS_ONE) return 0;
+    return (size_t)groups * win * sel_chunks(v) * (8 + 8 + 8 * (size_t)wout);
 }
+
+}  // extern "C"
+
+template <typename T>
+static int select_launch(const SelArgs& a, int32_t groups, void* work, hipStream_t st) {
+    const int64_t all = (int64_t)a.win * a.v;
+    if (all <= BS_ONE) {
+        // up to 16 candidates a thread; a few groups alone get 1,024 threads
+        const int nt = all > 4096 || (groups < 256 && all > 1024) ? 1024 : 256;
+        int parts = 1;
+        while (parts * 2 * a.win <= nt / 64) parts *= 2;
+        const size_t lds = ((size_t)(all + 1) / 2 * 2) * 4 + (size_t)a.wout * (nt / 64 + (all + nt - 1) / nt) * 8;
+        hipLaunchKernelGGL(beam_select_kernel<T>, dim3(groups), dim3(nt), lds, st, a, parts);
+        return HTM_OK;
+    }
+    SelWork k;
+    k.chunks = sel_chunks(a.v);
+    const int64_t rows = (int64_t)groups * a.win;
+    k.sum = (double*)work;
+    k.keys = (uint64_t*)(k.sum + rows * k.chunks);
+    k.top = (float*)(k.keys + rows * k.chunks * a.wout);
+    for (int64_t r0 = 0; r0 < rows; r0 += 65535) {
+        const dim3 grid(k.chunks, (uint32_t)(rows - r0 < 65535 ? rows - r0 : 65535));
+        hipLaunchKernelGGL(beam_sums_kernel<T>, grid, dim3(256), 0, st, a, k, r0);
+        hipLaunchKernelGGL(beam_chunk_kernel<T>, grid, dim3(256), 0, st, a, k, r0);
+    }
+    const int64_t keys = (int64_t)a.win * k.chunks * a.wout;
+    hipLaunchKernelGGL(beam_merge_kernel, dim3(groups), dim3(keys > 2048 ? 1024 : 256), 0, st, a, k);
+    return HTM_OK;
+}
+
+extern "C" {
 
 int htm_beam_select(const void* x, int32_t dtype, int64_t gs, int64_t bs, const float* score, const int32_t* live,
                     int32_t groups, int32_t win, int32_t wout, int32_t v, float* o_score, int32_t* o_parent,
                     int32_t* o_bucket, void* work, size_t work_bytes, void* stream) {
-    (void)work;
-    (void)work_bytes;
     if (groups < 0 || win < 1 || win > BS_MAX || wout < 1 || wout > BS_MAX || v < 1 || (int64_t)win * v >= 0x7FFFFFFFll)
         return htm_fail(HTM_E_INVALID, "%s: 1..64 beams in and out, outputs >= 1, beams_in * outputs < 2^31", __func__);
     if (dtype != HTM_T_F32 && dtype != HTM_T_F16 && dtype != HTM_T_BF16)
@@ -189,14 +496,14 @@ int htm_beam_select(const void* x, int32_t dtype, int64_t gs, int64_t bs, const 
     if (!groups) return HTM_OK;
     if (!x || !score || !o_score || !o_parent || !o_bucket || gs < 0 || bs < 0)
         return htm_fail(HTM_E_INVALID, "%s: invalid argument", __func__);
+    const size_t need = htm_beam_work_bytes(groups, win, wout, v);
+    if (need && (!work || (uintptr_t)work % 8 || work_bytes < need))
+        return htm_fail(HTM_E_INVALID, "%s: needs htm_beam_work_bytes of scratch, 8-byte aligned", __func__);
     const SelArgs a{x, gs, bs, score, live, win, wout, v, o_score, o_parent, o_bucket};
     hipStream_t st = (hipStream_t)stream;
-    if (dtype == HTM_T_F32)
-        hipLaunchKernelGGL(beam_select_kernel<float>, dim3(groups), dim3(BS_NT), 0, st, a);
-    else if (dtype == HTM_T_F16)
-        hipLaunchKernelGGL(beam_select_kernel<__half>, dim3(groups), dim3(BS_NT), 0, st, a);
-    else
-        hipLaunchKernelGGL(beam_select_kernel<__hip_bfloat16>, dim3(groups), dim3(BS_NT), 0, st, a);
+    if (dtype == HTM_T_F32) select_launch<float>(a, groups, work, st);
+    else if (dtype == HTM_T_F16) select_launch<__half>(a, groups, work, st);
+    else select_launch<__hip_bfloat16>(a, groups, work, st);
     return hipGetLastError() == hipSuccess ? HTM_OK : htm_fail(HTM_E_HIP, "beam select launch failed");
 }
 
