@@ -69,15 +69,15 @@ def beam_select(logits, scores, beams: int, live=None):
     return o_score, o_parent, o_bucket
 
 
-def _row_bytes(t, groups, beams):
-    if t.dim() >= 2 and t.shape[0] == groups and t.shape[1] == beams:
-        rows = groups * beams
-    elif t.dim() >= 1 and t.shape[0] == groups * beams:
-        rows = t.shape[0]
-    else:
-        raise ValueError("a buffer must be [groups * beams, ...] or [groups, beams, ...] for %d groups of %d, got %s" %
-                         (groups, beams, tuple(t.shape)))
-    return t.numel() * t.element_size() // rows if rows else 0
+_ARRAYS = {}
+
+
+def _arrays(n):
+    """ctypes arrays for n buffers: sources, destinations, row bytes."""
+    if n not in _ARRAYS:
+        _ARRAYS[n] = (ctypes.c_void_p * n, ctypes.c_size_t * n)
+    p, s = _ARRAYS[n]
+    return p(), p(), s()
 
 
 def beam_reorder(buffers, parent, out=None):
@@ -99,15 +99,22 @@ def beam_reorder(buffers, parent, out=None):
     if not 1 <= len(buffers) <= MAX_BUFFERS or len(dst) != len(buffers):
         raise ValueError("1..%d buffers and as many destinations" % MAX_BUFFERS)
     groups, beams = parent.shape
+    rows = groups * beams
     dev = parent.device
     parent = parent.contiguous()
     n = len(buffers)
-    src_p, dst_p, size = (ctypes.c_void_p * n)(), (ctypes.c_void_p * n)(), (ctypes.c_size_t * n)()
-    for k, (a, b) in enumerate(zip(buffers, dst)):
-        if not isinstance(a, torch.Tensor) or not isinstance(b, torch.Tensor) or a.device != dev or b.device != dev or \
-                a.dtype != b.dtype or a.shape != b.shape or not a.is_contiguous() or not b.is_contiguous():
+    src_p, dst_p, size = _arrays(n)
+    for k, a in enumerate(buffers):
+        b = dst[k]
+        if not isinstance(a, torch.Tensor) or a.device != dev or not a.is_contiguous() or b is not a and (
+                not isinstance(b, torch.Tensor) or b.device != dev or b.dtype != a.dtype or b.shape != a.shape or
+                not b.is_contiguous()):
             raise ValueError("buffers and destinations must be contiguous, alike, and on %s" % dev)
-        src_p[k], dst_p[k], size[k] = a.data_ptr(), b.data_ptr(), _row_bytes(a, groups, beams)
+        shape = a.shape
+        if not shape or shape[0] != rows and shape[:2] != (groups, beams):
+            raise ValueError("a buffer must be [groups * beams, ...] or [groups, beams, ...] for %d groups of %d, got %s" %
+                             (groups, beams, tuple(shape)))
+        src_p[k], dst_p[k], size[k] = a.data_ptr(), b.data_ptr(), a.nbytes // rows if rows else 0
     with _On(dev.index) as stream:
         check(L.htm_beam_reorder(n, src_p, dst_p, size, parent.data_ptr(), groups, beams, stream))
     return dst

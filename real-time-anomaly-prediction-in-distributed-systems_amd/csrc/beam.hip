@@ -373,74 +373,159 @@ __global__ void __launch_bounds__(1024) beam_merge_kernel(SelArgs a, SelWork k) 
 }
 
 // ------------------------------------------------------------------- rows
-// Out of place: a grid-stride copy in units of U, the row of each unit found
-// by division.
-template <typename U>
-__global__ void __launch_bounds__(256) rows_copy_kernel(const U* __restrict__ src, U* __restrict__ dst, uint64_t per,
-                                                        const int32_t* __restrict__ idx, int64_t n_rows, int beams,
-                                                        int64_t n_src) {
-    const uint64_t total = per * (uint64_t)n_rows;
-    for (uint64_t t = (uint64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (uint64_t)gridDim.x * 256) {
-        const uint64_t r = t / per, k = t - r * per;
-        int64_t from = idx[r];
-        if (beams) {
-            const int64_t w = (int64_t)(r % (uint64_t)beams);
-            from = (int64_t)r - w + (from >= 0 && from < beams ? from : w);
-        } else if (from < 0 || from >= n_src) {
-            continue;
-        }
-        dst[t] = src[(uint64_t)from * per + k];
-    }
-}
+// All buffers of a call in one launch: block b belongs to buffer k with first[k]
+// <= b < first[k + 1].  A buffer's rows are moved in its widest unit (16 bytes
+// down to 1, what its size and addresses divide by); 2^lanes[k] threads share a
+// row, four units each, all read before the first is written.
+struct MoveArgs {
+    RowMoves m;
+    uint32_t first[HTM_BEAM_BUFFERS + 1];
+    uint32_t units[HTM_BEAM_BUFFERS];   // of a row
+    uint8_t width[HTM_BEAM_BUFFERS];    // log2 of a unit's bytes
+    uint8_t lanes[HTM_BEAM_BUFFERS];
+    uint16_t parts[HTM_BEAM_BUFFERS];   // blocks side by side over a row
+    const int32_t* idx;
+    int64_t n_rows, n_src;
+    int32_t beams;
+};
 
-// In place: a thread owns one unit column of a group, reads it for every beam
-// and only then writes it, so no other thread's data is involved.
-template <typename U>
-__global__ void __launch_bounds__(256) rows_inplace_kernel(U* base, uint64_t per, const int32_t* __restrict__ idx,
-                                                           int64_t groups, int beams) {
-    const uint64_t total = per * (uint64_t)groups;
-    for (uint64_t t = (uint64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (uint64_t)gridDim.x * 256) {
-        const uint64_t g = t / per, k = t - g * per;
-        const int32_t* p = idx + g * (uint64_t)beams;
-        U* b = base + g * (uint64_t)beams * per + k;
-        U v[BS_MAX];
-#pragma unroll
-        for (int w = 0; w < BS_MAX; w++)
-            if (w < beams) {
-                const int q = p[w];
-                if (q >= 0 && q < beams && q != w) v[w] = b[(uint64_t)q * per];
-            }
-#pragma unroll
-        for (int w = 0; w < BS_MAX; w++)
-            if (w < beams) {
-                const int q = p[w];
-                if (q >= 0 && q < beams && q != w) b[(uint64_t)w * per] = v[w];
-            }
-    }
-}
+#define MOVE_UNITS 4
+typedef uint32_t unit16 __attribute__((ext_vector_type(4)));
+typedef uint32_t unit8 __attribute__((ext_vector_type(2)));
 
 template <typename U>
-static void rows_launch(const RowMoves& m, int k, const int32_t* idx, int64_t n_rows, int32_t beams, int64_t n_src,
-                        hipStream_t st) {
-    const uint64_t per = m.bytes[k] / sizeof(U);
-    const bool inplace = m.src[k] == m.dst[k];
-    const uint64_t total = per * (uint64_t)(inplace ? n_rows / beams : n_rows);
-    const uint64_t wg = (total + 255) / 256;
-    const dim3 grid((uint32_t)(wg < 65536 ? wg : 65536));
-    if (inplace)
-        hipLaunchKernelGGL(rows_inplace_kernel<U>, grid, dim3(256), 0, st, (U*)m.dst[k], per, idx, n_rows / beams, beams);
-    else
-        hipLaunchKernelGGL(rows_copy_kernel<U>, grid, dim3(256), 0, st, (const U*)m.src[k], (U*)m.dst[k], per, idx,
-                           n_rows, beams, n_src);
+__device__ __forceinline__ void move_out(const MoveArgs& a, int k, uint32_t block) {
+    const int log = a.lanes[k], t = threadIdx.x & ((1 << log) - 1);
+    const uint32_t units = a.units[k], parts = a.parts[k];
+    const uint32_t row_block = parts == 1 ? block : block / parts, part = block - row_block * parts;
+    const int64_t r = ((int64_t)row_block << (8 - log)) + (threadIdx.x >> log);
+    if (r >= a.n_rows) return;
+    int64_t from = a.idx[r];
+    if (a.beams) {
+        const int64_t w = a.n_rows <= 0xFFFFFFFFll ? (int64_t)((uint32_t)r % (uint32_t)a.beams) : r % a.beams;
+        from = r - w + (from >= 0 && from < a.beams ? from : w);
+    } else if (from < 0 || from >= a.n_src) {
+        return;
+    }
+    const U* src = reinterpret_cast<const U*>(a.m.src[k]) + from * (int64_t)units;
+    U* dst = reinterpret_cast<U*>(a.m.dst[k]) + r * (int64_t)units;
+    const uint32_t u0 = part * (MOVE_UNITS * 256) + t;
+    U v[MOVE_UNITS];
+#pragma unroll
+    for (int j = 0; j < MOVE_UNITS; j++)
+        if (u0 + (j << log) < units) v[j] = src[u0 + (j << log)];
+#pragma unroll
+    for (int j = 0; j < MOVE_UNITS; j++)
+        if (u0 + (j << log) < units) dst[u0 + (j << log)] = v[j];
+}
+
+__device__ __forceinline__ int move_buffer(const MoveArgs& a) {
+    int k = 0;
+    while (blockIdx.x >= a.first[k + 1]) k++;
+    return k;
+}
+
+// Blocks go to the chip's 8 XCDs in turn; each takes a run of neighbouring rows,
+// so that a parent of several rows of a group is read from memory once, into
+// the L2 of the XCD that copies the group.
+__device__ __forceinline__ uint32_t near_block(uint32_t b, uint32_t n) {
+    const uint32_t q = n / 8, r = n % 8, x = b % 8, i = b / 8;
+    return x * q + min(x, r) + i;
+}
+
+__global__ void __launch_bounds__(256) rows_copy_kernel(MoveArgs a) {
+    const int k = move_buffer(a);
+    const uint32_t b = near_block(blockIdx.x - a.first[k], a.first[k + 1] - a.first[k]);
+    if (a.width[k] == 4) move_out<unit16>(a, k, b);
+    else if (a.width[k] == 3) move_out<unit8>(a, k, b);
+    else if (a.width[k] == 2) move_out<uint32_t>(a, k, b);
+    else if (a.width[k] == 1) move_out<uint16_t>(a, k, b);
+    else move_out<uint8_t>(a, k, b);
+}
+
+// In place: a thread owns a unit's place in all W rows of a group, reads the
+// parents' and only then writes, so that no other thread's data is involved and
+// nothing is kept beside the buffers.  Rows that stay are not touched.
+template <typename U, int W>
+__device__ __forceinline__ void move_in(const MoveArgs& a, int k, uint32_t block) {
+    const int log = a.lanes[k], t = threadIdx.x & ((1 << log) - 1);
+    const uint32_t units = a.units[k], parts = a.parts[k];
+    const uint32_t row_block = parts == 1 ? block : block / parts, part = block - row_block * parts;
+    const int64_t g = ((int64_t)row_block << (8 - log)) + (threadIdx.x >> log);
+    const uint32_t u = part * 256 + t;
+    if (g >= a.n_rows / a.beams || u >= units) return;
+    const int32_t* p = a.idx + g * a.beams;
+    U* b = reinterpret_cast<U*>(a.m.dst[k]) + g * a.beams * (int64_t)units + u;
+    // (a row that stays reads row 0 instead: a read without a branch, of a row that is read at most once more)
+    U v[W];
+    uint64_t moved = 0;
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+        const int q = w < a.beams ? p[w] : w;
+        const bool go = q >= 0 && q < a.beams && q != w;
+        moved |= (uint64_t)go << w;
+        v[w] = b[(uint64_t)(go ? (uint32_t)q : 0u) * units];
+    }
+#pragma unroll
+    for (int w = 0; w < W; w++)
+        if ((moved >> w) & 1) b[(uint64_t)w * units] = v[w];
+}
+
+template <int W>
+__global__ void __launch_bounds__(256, W <= 8 ? 8 : W <= 16 ? 5 : W <= 32 ? 3 : 2) rows_inplace_kernel(MoveArgs a) {
+    const int k = move_buffer(a);
+    const uint32_t b = blockIdx.x - a.first[k];
+    if (W <= 32 && a.width[k] == 4) move_in<unit16, (W <= 32 ? W : 1)>(a, k, b);
+    else if (a.width[k] == 3) move_in<unit8, W>(a, k, b);
+    else if (a.width[k] == 2) move_in<uint32_t, W>(a, k, b);
+    else if (a.width[k] == 1) move_in<uint16_t, W>(a, k, b);
+    else move_in<uint8_t, W>(a, k, b);
 }
 
 int rows_move(const RowMoves& m, const int32_t* idx, int64_t n_rows, int32_t beams, int64_t n_src, hipStream_t st) {
     if (!n_rows) return HTM_OK;
-    for (int k = 0; k < m.n; k++) {
-        if (!m.bytes[k]) continue;
-        const uint64_t a = m.bytes[k] | (uint64_t)(uintptr_t)m.src[k] | (uint64_t)(uintptr_t)m.dst[k];
-        if (a % 4 == 0) rows_launch<uint32_t>(m, k, idx, n_rows, beams, n_src, st);
-        else rows_launch<uint8_t>(m, k, idx, n_rows, beams, n_src, st);
+    for (int inplace = 0; inplace < (beams ? 2 : 1); inplace++) {  // (an index of rows, beams 0, never moves in place)
+        MoveArgs a;
+        a.m.n = 0;
+        a.idx = idx;
+        a.n_rows = n_rows;
+        a.n_src = n_src;
+        a.beams = beams;
+        uint64_t blocks = 0;
+        const int64_t items = inplace ? n_rows / beams : n_rows;
+        for (int k = 0; k < m.n; k++) {
+            if (!m.bytes[k] || (m.src[k] == m.dst[k]) != (inplace != 0)) continue;
+            const int i = a.m.n++;
+            a.m.src[i] = m.src[k];
+            a.m.dst[i] = m.dst[k];
+            a.m.bytes[i] = m.bytes[k];
+            const uint64_t all = m.bytes[k] | (uint64_t)(uintptr_t)m.src[k] | (uint64_t)(uintptr_t)m.dst[k];
+            // (64 beams in place: 8-byte units keep a thread's rows in 128 registers)
+            int width = inplace && beams > 32 ? 3 : 4;
+            while (width && all & ((1ull << width) - 1)) width--;
+            const uint64_t units = m.bytes[k] >> width, per = inplace ? 1 : MOVE_UNITS;
+            int lanes = 0;
+            while (lanes < 8 && (per << lanes) < units) lanes++;
+            const uint64_t parts = (units + (per << 8) - 1) / (per << 8);
+            const uint64_t add = (((uint64_t)items + (256u >> lanes) - 1) >> (8 - lanes)) * parts;
+            if (units > 0xFFFFFFFFull || parts > 0xFFFFull || blocks + add > 0xFFFFFFull)
+                return htm_fail(HTM_E_INVALID, "rows of %llu bytes x %lld are more than one launch moves",
+                                (unsigned long long)m.bytes[k], (long long)n_rows);
+            a.units[i] = (uint32_t)units;
+            a.width[i] = (uint8_t)width;
+            a.lanes[i] = (uint8_t)lanes;
+            a.parts[i] = (uint16_t)parts;
+            a.first[i] = (uint32_t)blocks;
+            blocks += add;
+            a.first[i + 1] = (uint32_t)blocks;
+        }
+        if (!blocks) continue;
+        const dim3 grid((uint32_t)blocks);
+        if (!inplace) hipLaunchKernelGGL(rows_copy_kernel, grid, dim3(256), 0, st, a);
+        else if (beams <= 8) hipLaunchKernelGGL(rows_inplace_kernel<8>, grid, dim3(256), 0, st, a);
+        else if (beams <= 16) hipLaunchKernelGGL(rows_inplace_kernel<16>, grid, dim3(256), 0, st, a);
+        else if (beams <= 32) hipLaunchKernelGGL(rows_inplace_kernel<32>, grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL(rows_inplace_kernel<64>, grid, dim3(256), 0, st, a);
     }
     return hipGetLastError() == hipSuccess ? HTM_OK : htm_fail(HTM_E_HIP, "row move launch failed");
 }
