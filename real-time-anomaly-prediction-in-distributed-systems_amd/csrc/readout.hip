@@ -576,7 +576,15 @@ static int q4_bitmap(const htm_q4_shape* s, const void* rec, const uint32_t* pat
 #define Q4_GRID_Y 65535  // rows of one launch
 
 // How a product is shared out: NX rows at a time, runs of half blocks and ranges
-// of inputs.
+// of inputs, some 512 workgroups in all.  Measured, us (runs x ranges, both
+// launches; rows, inputs, outputs):
+//   8, 24,576, 7 x 480: 7 x 73 44, 7 x 36 50, 14 x 36 47, 4 x 64 58
+//   8, 24,576, 480: 2 x 128 20, 1 x 128 23, 1 x 64 30
+//   12, 4,000, 7 x 480: 14 x 16 22, 7 x 32 23, 7 x 8 38, 210 x 1 57
+//   8, 1,000, 7 x 500: 14 x 4 17, 7 x 8 18, 112 x 1 26
+//   1, 4,000, 480: 2 x 16 9.3, 30 x 1 12.5
+// In one launch while a tile holds the inputs (1, 300, 1,000: 16 x 1 5.7, 4 x 4
+// 7.1; 1, 2,048 with 6 % not zero, 480: 10 x 1 5.9, 2 x 8 7.0).
 struct MvPlan {
     int nx, passes, cb, chunks, splits, range;
 };
@@ -588,11 +596,14 @@ static MvPlan mv_plan(const Q4Dims& d, int per) {
     const int64_t y = (int64_t)d.nm * p.passes;
     const int halves = d.nh * d.nblk * 2;
     p.splits = 1;
-    if (d.ni <= 4096) {
-        p.chunks = (int)std::min<int64_t>(halves, std::max<int64_t>((halves + 31) / 32, 256 / y));
+    const int64_t few = 512;
+    if ((d.ni <= 256 || (per == 1 && d.ni <= 2048)) && (halves + 3) / 4 * y <= few) {
+        p.chunks = (halves + 3) / 4;
     } else {
-        p.chunks = (halves + 31) / 32;
-        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(512 / (p.chunks * y), d.ni / 256));
+        const int64_t most = (d.ni + 255) / 256;
+        p.chunks = (halves + 15) / 16;
+        if (p.chunks * most * y > few) p.chunks = (halves + 31) / 32;
+        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(few / (p.chunks * y), most));
     }
     p.cb = (halves + p.chunks - 1) / p.chunks;
     p.chunks = (halves + p.cb - 1) / p.cb;
