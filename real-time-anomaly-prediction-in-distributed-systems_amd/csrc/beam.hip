@@ -7,6 +7,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "beam_dev.h"
 #include "htm_dev.h"
 
@@ -34,36 +36,43 @@ __device__ __forceinline__ uint64_t make_key(uint32_t bits, uint32_t place) {
     return bits ? ((uint64_t)bits << 32) | (0xFFFFFFFFu - place) : 0;
 }
 
-// 2^t for t <= 0, relative error below 2^-46: the Taylor series of exp to degree
-// 11 on |f ln 2| <= 0.347 (remainder 0.347^12 / 12! = 6e-15).  A rounding border
-// of a float32 score is then missed once in some 10^6 candidates by one step,
-// as any other order of the same float64 sum would miss it.
-__device__ __forceinline__ double exp2_neg(double t) {
-    const double n = rint(t), f = (t - n) * 0.69314718055994530942;
-    double p = 1.0 / 39916800.0;
-    p = fma(p, f, 1.0 / 3628800.0);
-    p = fma(p, f, 1.0 / 362880.0);
-    p = fma(p, f, 1.0 / 40320.0);
-    p = fma(p, f, 1.0 / 5040.0);
-    p = fma(p, f, 1.0 / 720.0);
-    p = fma(p, f, 1.0 / 120.0);
-    p = fma(p, f, 1.0 / 24.0);
-    p = fma(p, f, 1.0 / 6.0);
-    p = fma(p, f, 0.5);
+// exp(x - m) for finite m >= x, x = -infinity included (0): 2^t as 2^n 2^f, |f| <=
+// 1/2, the Taylor series of 2^f to degree 10 (remainder (ln 2 / 2)^11 / 11! =
+// 2e-13).  A beam's sum off by that much moves a float32 score over a rounding
+// border, by one step, once in some 10^6 candidates, as any other order of the
+// same float64 sum does once in 10^9.
+__device__ __forceinline__ double exp_diff(float x, double m) {
+    const double t = fmax(((double)x - m) * 1.4426950408889634074, -1100.0);
+    const double n = rint(t), f = t - n;
+    double p = 7.0549116208011233e-9;       // ln(2)^k / k!, k = 10 ... 1
+    p = fma(p, f, 1.0178086009239699e-7);
+    p = fma(p, f, 1.3215486790144309e-6);
+    p = fma(p, f, 1.5252733804059841e-5);
+    p = fma(p, f, 1.5403530393381610e-4);
+    p = fma(p, f, 1.3333558146428443e-3);
+    p = fma(p, f, 9.6181291076284772e-3);
+    p = fma(p, f, 5.5504108664821580e-2);
+    p = fma(p, f, 2.4022650695910071e-1);
+    p = fma(p, f, 6.9314718055994531e-1);
     p = fma(p, f, 1.0);
-    p = fma(p, f, 1.0);
-    return ldexp(p, (int)fmax(n, -2000.0));
-}
-
-// exp(x - m) of float32 numbers; x = -inf gives 0, a NaN or x - m = NaN gives NaN
-__device__ __forceinline__ double exp_diff(float x, float m) {
-    const double t = ((double)x - (double)m) * 1.4426950408889634074;
-    return t > -1100.0 ? exp2_neg(t) : (t == t ? 0.0 : t);
+    return ldexp(p, (int)n);
 }
 
 __device__ __forceinline__ float wave_max(float v) {
-    for (int k = 32; k; k >>= 1) v = fmaxf(v, __shfl_xor(v, k));
-    return v;
+    // lanes that a move does not reach take -infinity
+    const auto step = [&](auto ctrl, auto rows) {
+        const float o = __int_as_float(__builtin_amdgcn_update_dpp((int)0xFF800000, __float_as_int(v), decltype(ctrl)::value,
+                                                                   decltype(rows)::value, 0xF, false));
+        v = fmaxf(v, o);
+    };
+    using std::integral_constant;
+    step(integral_constant<int, 0x111>(), integral_constant<int, 0xF>());  // row_shr 1, 2, 4, 8
+    step(integral_constant<int, 0x112>(), integral_constant<int, 0xF>());
+    step(integral_constant<int, 0x114>(), integral_constant<int, 0xF>());
+    step(integral_constant<int, 0x118>(), integral_constant<int, 0xF>());
+    step(integral_constant<int, 0x142>(), integral_constant<int, 0xA>());  // row_bcast 15, 31
+    step(integral_constant<int, 0x143>(), integral_constant<int, 0xC>());
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
 __device__ __forceinline__ double wave_sum(double v) {
@@ -76,42 +85,36 @@ struct TopSh {
     uint32_t count;  // candidates that reach it
 };
 
-// The best `want` (<= 64) of the candidates held in LDS: bits[0..n), places place0
-// + index, nt = blockDim.x threads, tops: room for want keys a wave, list: for
-// want * ceil(n / nt) keys.
-// Every thread's best candidate first; the want-th best of those is a floor that
-// at least `want` candidates reach (or all there are), and at most want threads
-// hold any that do, so a short list is left, whose members count those before
-// them.  put(rank, key) is called once for each candidate taken.  Every step is
-// a comparison of distinct keys: the result does not depend on the order in
-// which the list was filled.
-template <typename PUT>
-__device__ __forceinline__ void top_of(const uint32_t* bits, int n, uint32_t place0, int want, TopSh& sh, uint64_t* tops,
-                                       uint64_t* list, PUT put) {
+// The best `want` (<= 64) of a workgroup's candidates.  mine: the thread's best
+// key (0: none); each(f): f(key) for every candidate of the thread; tops: LDS for
+// want keys a wave, list: for want times the most candidates that a thread has.
+// The want-th best of the threads' best is a floor that at least `want`
+// candidates reach (or all there are), and at most want threads hold any that
+// do, so a short list is left, whose members count those before them.
+// put(rank, key) is called once for each candidate taken.  Every step is a
+// comparison of distinct keys: the result does not depend on the order in which
+// the list was filled.
+template <typename EACH, typename PUT>
+__device__ __forceinline__ void top_of(uint64_t mine, int want, TopSh& sh, uint64_t* tops, uint64_t* list, EACH each, PUT put) {
     const int nt = blockDim.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nwave = nt >> 6;
-    uint32_t best = 0, at = 0;
-    for (int i = threadIdx.x; i < n; i += nt) {
-        const uint32_t b = bits[i];
-        if (b > best) best = b, at = i;
-    }
-    const uint64_t mine = make_key(best, place0 + at);
     if (want >= 64) {
         tops[threadIdx.x] = mine;
     } else {
-        uint32_t cur = best;
+        uint32_t hi = (uint32_t)(mine >> 32);
+        const uint32_t lo = (uint32_t)mine;
         uint64_t won = 0;  // lane r: the wave's r-th best
         for (int r = 0; r < want; r++) {
-            const uint32_t top = wave_max_u32(cur);
+            const uint32_t top = wave_max_u32(hi);
             if (!top) break;
-            uint64_t eq = __ballot(cur == top);
-            if (eq & (eq - 1)) {  // equal scores: the lowest place of them
-                const uint32_t low = ~wave_max_u32(cur == top ? ~at : 0u);
-                eq = __ballot(cur == top && at == low);
+            uint64_t eq = __ballot(hi == top);
+            if (eq & (eq - 1)) {  // equal scores: the lowest place, the largest lower word
+                const uint32_t low = wave_max_u32(hi == top ? lo : 0u);
+                eq = __ballot(hi == top && lo == low);
             }
             const int src = __ffsll((unsigned long long)eq) - 1;
-            const uint32_t p = (uint32_t)__builtin_amdgcn_readlane((int)at, src);
-            if (lane == r) won = make_key(top, place0 + p);
-            if (lane == src) cur = 0;
+            const uint32_t p = (uint32_t)__builtin_amdgcn_readlane((int)lo, src);
+            if (lane == r) won = ((uint64_t)top << 32) | p;
+            if (lane == src) hi = 0;
         }
         if (lane < want) tops[wave * want + lane] = won;
     }
@@ -130,10 +133,9 @@ __device__ __forceinline__ void top_of(const uint32_t* bits, int n, uint32_t pla
     __syncthreads();
     const uint64_t floor = sh.floor;
     if (mine >= floor)
-        for (int i = threadIdx.x; i < n; i += nt) {
-            const uint64_t k = make_key(bits[i], place0 + (uint32_t)i);
+        each([&](uint64_t k) {
             if (k >= floor) list[atomicAdd(&sh.count, 1u)] = k;
-        }
+        });
     __syncthreads();
     const int m = (int)sh.count;
     for (int i = threadIdx.x; i < m; i += nt) {
@@ -182,67 +184,92 @@ __device__ __forceinline__ void put_rest(const SelArgs& a, int64_t g, int taken)
 template <typename T>
 __global__ void __launch_bounds__(1024) beam_select_kernel(SelArgs a, int parts) {
     __shared__ TopSh sh;
-    __shared__ double sum[BS_MAX];  // [beam * parts + part]: parts > 1 only while beams * parts <= waves
+    __shared__ double sum[BS_MAX];   // [beam * parts + part]: parts > 1 only while beams * parts <= waves
     __shared__ float top[BS_MAX];
-    extern __shared__ __attribute__((aligned(16))) uint32_t cand[];  // [win * v] logits, then score bits; tops; list
+    __shared__ double base[BS_MAX];  // a beam's score - log(sum); NaN: none of its continuations counts
+    __shared__ double largest[BS_MAX];  // its largest logit
+    extern __shared__ __attribute__((aligned(16))) float cand[];  // [win * v] logits, then scores; tops; list
     const int64_t g = blockIdx.x;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nwave = blockDim.x >> 6;
-    const int n = live_of(a, g), rows = nwave / parts, part = wave % parts;
+    const int n = live_of(a, g), rows = nwave / parts, part = wave % parts, first = wave / parts;
     const T* x = (const T*)a.x + g * a.gs;
-    const int step = parts * 64;
-    for (int w = wave / parts; w < a.win; w += rows) {
+    const int step = parts * 64, o0 = part * 64 + lane;
+    for (int w = first; w < a.win; w += rows) {
         const T* p = x + (int64_t)w * a.bs;
-        uint32_t* c = cand + w * a.v;
+        float* c = cand + w * a.v;
         float m = -INFINITY;
-        int o = part * 64 + lane;
+        bool nan = false;
+        int o = o0;
         for (; o + 7 * step < n; o += 8 * step) {
             float v[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) v[j] = up(p[o + j * step]);
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                c[o + j * step] = __float_as_uint(v[j]);
+                c[o + j * step] = v[j];
                 m = fmaxf(m, v[j]);
+                nan |= v[j] != v[j];
             }
         }
 #pragma unroll 4
         for (; o < n; o += step) {
             const float v = up(p[o]);
-            c[o] = __float_as_uint(v);
+            c[o] = v;
             m = fmaxf(m, v);
+            nan |= v != v;
         }
         m = wave_max(m);
-        if (lane == 0) top[w * parts + part] = m;
+        const bool spoilt = __ballot(nan) != 0;  // (a NaN spoils the beam as +infinity does)
+        if (lane == 0) top[w * parts + part] = spoilt ? INFINITY : m;
     }
     __syncthreads();
-    for (int w = wave / parts; w < a.win; w += rows) {
+    for (int w = first; w < a.win; w += rows) {
         float m = top[w * parts];
         for (int k = 1; k < parts; k++) m = fmaxf(m, top[w * parts + k]);
-        const uint32_t* c = cand + w * a.v;
+        const float* c = cand + w * a.v;
+        const double md = (double)m;
         double s = 0.0;
-#pragma unroll 2
-        for (int o = part * 64 + lane; o < n; o += step) s += exp_diff(__uint_as_float(c[o]), m);
+        if (fabsf(m) < INFINITY) {
+#pragma unroll 4
+            for (int o = o0; o < n; o += step) s += exp_diff(c[o], md);
+        }
         s = wave_sum(s);
         if (lane == 0) sum[w * parts + part] = s;
     }
     __syncthreads();
-    for (int w = wave / parts; w < a.win; w += rows) {
+    if ((int)threadIdx.x < a.win) {
+        const int w = threadIdx.x;
         float m = top[w * parts];
         double s = sum[w * parts];
         for (int k = 1; k < parts; k++) {
             m = fmaxf(m, top[w * parts + k]);
             s += sum[w * parts + k];
         }
-        // (no finite logit, an infinite one or a NaN: the sum is 0 or NaN, and no score of the beam is a number)
-        const double base = (double)a.score[g * a.win + w] - log(s);
-        uint32_t* c = cand + w * a.v;
-        for (int o = part * 64 + lane; o < a.v; o += step)
-            c[o] = o < n ? score_bits((float)(((double)__uint_as_float(c[o]) - (double)m) + base)) : 0u;
+        largest[w] = (double)m;
+        // (no finite logit, an infinite one or a NaN: no score of the beam is a number)
+        base[w] = fabsf(m) < INFINITY ? (double)a.score[g * a.win + w] - log(s) : (double)NAN;
     }
     __syncthreads();
+    float best = -INFINITY;
+    uint32_t at = 0;
+    for (int w = first; w < a.win; w += rows) {
+        const double b = base[w], m = largest[w];
+        float* c = cand + w * a.v;
+#pragma unroll 4
+        for (int o = o0; o < n; o += step) {
+            const float v = (float)(((double)c[o] - m) + b);
+            c[o] = v;
+            if (v > best) best = v, at = (uint32_t)(w * a.v + o);
+        }
+    }
     const int all = a.win * a.v;
     uint64_t* tops = reinterpret_cast<uint64_t*>(cand + ((all + 1) & ~1));
-    top_of(cand, all, 0, a.wout, sh, tops, tops + nwave * a.wout, [&](int r, uint64_t k) { put_key(a, g, r, k); });
+    const auto each = [&](auto f) {
+        for (int w = first; w < a.win; w += rows)
+            for (int o = o0; o < n; o += step) f(make_key(score_bits(cand[w * a.v + o]), (uint32_t)(w * a.v + o)));
+    };
+    top_of(make_key(score_bits(best), at), a.wout, sh, tops, tops + nwave * a.wout, each,
+           [&](int r, uint64_t k) { put_key(a, g, r, k); });
     __syncthreads();
     put_rest(a, g, min((int)sh.count, a.wout));
 }
@@ -250,7 +277,7 @@ __global__ void __launch_bounds__(1024) beam_select_kernel(SelArgs a, int parts)
 // Many candidates: chunks of BS_CHUNK of a beam's outputs, three launches.
 #define BS_CHUNK 4096
 struct SelWork {
-    float* top;      // [groups * win * chunks] the chunks' largest logits
+    float* top;      // [groups * win * chunks] the chunks' largest logits, +infinity where there is a NaN
     double* sum;     // ... and sums of exp(x - top)
     uint64_t* keys;  // [groups * win * chunks * wout] the chunks' best
     int32_t chunks;
@@ -264,20 +291,27 @@ __global__ void __launch_bounds__(256) beam_sums_kernel(SelArgs a, SelWork k, in
     const int o0 = blockIdx.x * BS_CHUNK, n = min(live_of(a, g), o0 + BS_CHUNK);
     const T* p = (const T*)a.x + g * a.gs + (row - g * a.win) * a.bs;
     float v[BS_CHUNK / 256], m = -INFINITY;
+    bool nan = false;
 #pragma unroll
     for (int j = 0; j < BS_CHUNK / 256; j++) {
         const int o = o0 + j * 256 + threadIdx.x;
         v[j] = o < n ? up(p[o]) : -INFINITY;
-        m = fmaxf(m, v[j]);
     }
-    m = wave_max(m);
+#pragma unroll
+    for (int j = 0; j < BS_CHUNK / 256; j++) {
+        m = fmaxf(m, v[j]);
+        nan |= v[j] != v[j];
+    }
+    m = wave_max(nan ? INFINITY : m);
     if ((threadIdx.x & 63) == 0) tm[threadIdx.x >> 6] = m;
     __syncthreads();
     m = fmaxf(fmaxf(tm[0], tm[1]), fmaxf(tm[2], tm[3]));
+    const double md = (double)m;
     double s = 0.0;
-#pragma unroll
-    for (int j = 0; j < BS_CHUNK / 256; j++)
-        if (o0 + j * 256 + (int)threadIdx.x < n) s += m > -INFINITY ? exp_diff(v[j], m) : v[j] == v[j] ? 0.0 : (double)v[j];
+    if (fabsf(m) < INFINITY) {
+#pragma unroll 4
+        for (int j = 0; j < BS_CHUNK / 256; j++) s += exp_diff(v[j], md);
+    }
     s = wave_sum(s);
     if ((threadIdx.x & 63) == 0) ts[threadIdx.x >> 6] = s;
     __syncthreads();
@@ -290,7 +324,6 @@ __global__ void __launch_bounds__(256) beam_sums_kernel(SelArgs a, SelWork k, in
 template <typename T>
 __global__ void __launch_bounds__(256) beam_chunk_kernel(SelArgs a, SelWork k, int64_t row0) {
     __shared__ TopSh sh;
-    __shared__ uint32_t cand[BS_CHUNK];
     __shared__ uint64_t tops[BS_MAX * 4], list[BS_MAX * (BS_CHUNK / 256)];
     __shared__ float tm[4];
     __shared__ double ts[4];
@@ -313,49 +346,63 @@ __global__ void __launch_bounds__(256) beam_chunk_kernel(SelArgs a, SelWork k, i
     if (lane == 0) tm[wave] = m;
     __syncthreads();
     m = fmaxf(fmaxf(tm[0], tm[1]), fmaxf(tm[2], tm[3]));
+    const double md = (double)m;
     double s = 0.0;
-    for (int c = threadIdx.x; c < k.chunks; c += 256)
-        if (top[c] > -INFINITY || sum[c] != 0.0) s += sum[c] * exp_diff(top[c], m);  // (a chunk without a live output adds nothing)
+    if (fabsf(m) < INFINITY)
+        for (int c = threadIdx.x; c < k.chunks; c += 256) s += sum[c] * exp_diff(top[c], md);
     s = wave_sum(s);
     if (lane == 0) ts[wave] = s;
     __syncthreads();
     s = (ts[0] + ts[1]) + (ts[2] + ts[3]);
-    const double base = (double)a.score[row] - log(s);
+    const double base = fabsf(m) < INFINITY ? (double)a.score[row] - log(s) : (double)NAN;
+    float best = -INFINITY;
+    uint32_t at = 0;
+    const uint32_t place0 = (uint32_t)(w * (int64_t)a.v + o0);
 #pragma unroll
     for (int j = 0; j < BS_CHUNK / 256; j++) {
-        const int i = j * 256 + threadIdx.x;
-        cand[i] = o0 + i < n ? score_bits((float)(((double)v[j] - (double)m) + base)) : 0u;
+        v[j] = (float)(((double)v[j] - md) + base);  // (behind the live outputs: -infinity or NaN)
+        if (v[j] > best) best = v[j], at = place0 + j * 256 + threadIdx.x;
     }
-    __syncthreads();
     uint64_t* keys = k.keys + (row * k.chunks + blockIdx.x) * a.wout;
-    top_of(cand, BS_CHUNK, (uint32_t)(w * (int64_t)a.v + o0), a.wout, sh, tops, list, [&](int r, uint64_t key) { keys[r] = key; });
+    const auto each = [&](auto f) {
+#pragma unroll
+        for (int j = 0; j < BS_CHUNK / 256; j++) f(make_key(score_bits(v[j]), place0 + j * 256 + threadIdx.x));
+    };
+    top_of(make_key(score_bits(best), at), a.wout, sh, tops, list, each, [&](int r, uint64_t key) { keys[r] = key; });
     __syncthreads();
     for (int r = (int)sh.count + (int)threadIdx.x; r < a.wout; r += 256) keys[r] = 0;
 }
 
-// The chunks' best of one group: each thread its own of the keys, the best key
-// below the last one taken, wout times.
+// The chunks' best of one group: the best of them.  A thread has at most `held`
+// keys (list: wout * held in dynamic LDS, behind the waves' tops).
 __global__ void __launch_bounds__(1024) beam_merge_kernel(SelArgs a, SelWork k) {
-    __shared__ uint64_t red[16];
-    const int64_t g = blockIdx.x;
-    const int64_t n = (int64_t)a.win * k.chunks * a.wout;
+    __shared__ TopSh sh;
+    extern __shared__ __attribute__((aligned(16))) uint64_t lds[];
+    const int64_t g = blockIdx.x, n = (int64_t)a.win * k.chunks * a.wout;
     const uint64_t* keys = k.keys + g * n;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nwave = blockDim.x >> 6;
-    constexpr int HELD = 8;  // keys of a thread in registers; any more are read again
-    uint64_t mine[HELD];
-#pragma unroll
-    for (int j = 0; j < HELD; j++) {
-        const int64_t i = (int64_t)j * blockDim.x + threadIdx.x;
-        mine[j] = i < n ? keys[i] : 0;
-    }
+    uint64_t best = 0;
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) best = keys[i] > best ? keys[i] : best;
+    const auto each = [&](auto f) {
+        for (int64_t i = threadIdx.x; i < n; i += blockDim.x) f(keys[i]);
+    };
+    top_of(best, a.wout, sh, lds, lds + (blockDim.x >> 6) * a.wout, each, [&](int r, uint64_t key) { put_key(a, g, r, key); });
+    __syncthreads();
+    put_rest(a, g, min((int)sh.count, a.wout));
+}
+
+// The same for so many chunks that such a list does not fit: the best key below
+// the last one taken, wout times.
+__global__ void __launch_bounds__(1024) beam_merge_many_kernel(SelArgs a, SelWork k) {
+    __shared__ uint64_t red[16];
+    const int64_t g = blockIdx.x, n = (int64_t)a.win * k.chunks * a.wout;
+    const uint64_t* keys = k.keys + g * n;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint64_t prev = ~0ull;
     int r = 0;
     for (; r < a.wout; r++) {
         uint64_t best = 0;
-#pragma unroll
-        for (int j = 0; j < HELD; j++)
-            if (mine[j] < prev && mine[j] > best) best = mine[j];
-        for (int64_t i = (int64_t)HELD * blockDim.x + threadIdx.x; i < n; i += blockDim.x)
+        for (int64_t i = threadIdx.x; i < n; i += 1024)
             if (keys[i] < prev && keys[i] > best) best = keys[i];
         // the upper word's largest, then the lower word's among those
         const uint32_t hi = wave_max_u32((uint32_t)(best >> 32));
@@ -363,7 +410,7 @@ __global__ void __launch_bounds__(1024) beam_merge_kernel(SelArgs a, SelWork k) 
         if (lane == 0) red[wave] = ((uint64_t)hi << 32) | lo;
         __syncthreads();
         best = 0;
-        for (int j = 0; j < nwave; j++) best = red[j] > best ? red[j] : best;
+        for (int j = 0; j < 16; j++) best = red[j] > best ? red[j] : best;
         __syncthreads();
         if (!(best >> 32)) break;
         if (threadIdx.x == 0) put_key(a, g, r, best);
@@ -565,7 +612,10 @@ static int select_launch(const SelArgs& a, int32_t groups, void* work, hipStream
         hipLaunchKernelGGL(beam_chunk_kernel<T>, grid, dim3(256), 0, st, a, k, r0);
     }
     const int64_t keys = (int64_t)a.win * k.chunks * a.wout;
-    hipLaunchKernelGGL(beam_merge_kernel, dim3(groups), dim3(keys > 2048 ? 1024 : 256), 0, st, a, k);
+    const int nt = keys > 2048 ? 1024 : 256;
+    const int64_t lds = 8 * (int64_t)a.wout * (nt / 64 + (keys + nt - 1) / nt);
+    if (lds <= 60 * 1024) hipLaunchKernelGGL(beam_merge_kernel, dim3(groups), dim3(nt), (size_t)lds, st, a, k);
+    else hipLaunchKernelGGL(beam_merge_many_kernel, dim3(groups), dim3(1024), 0, st, a, k);
     return HTM_OK;
 }
 
