@@ -57,9 +57,8 @@ def beam_select(logits, scores, beams: int, live=None):
     scores = scores.contiguous()
     live = live.contiguous() if live is not None else None
     with _On(dev.index) as stream:
-        o_score = torch.empty((groups, beams), dtype=torch.float32, device=dev)
-        o_parent = torch.empty((groups, beams), dtype=torch.int32, device=dev)
-        o_bucket = torch.empty((groups, beams), dtype=torch.int32, device=dev)
+        o_score, o_parent, o_bucket = scores.new_empty((3, groups, beams), dtype=torch.int32).unbind(0)
+        o_score = o_score.view(torch.float32)
         nb = L.htm_beam_work_bytes(groups, win, beams, v)
         work = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
         check(L.htm_beam_select(logits.data_ptr(), code, gs, bs, scores.data_ptr(),

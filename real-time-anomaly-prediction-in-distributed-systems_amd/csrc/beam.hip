@@ -76,74 +76,109 @@ __device__ __forceinline__ float wave_max(float v) {
 }
 
 __device__ __forceinline__ double wave_sum(double v) {
-    for (int k = 32; k; k >>= 1) v += __shfl_xor(v, k);
-    return v;
+    // lanes that a move does not reach take 0
+    const auto step = [&](auto ctrl, auto rows) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, decltype(ctrl)::value,
+                                                                  decltype(rows)::value, 0xF, false);
+        const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), decltype(ctrl)::value,
+                                                                  decltype(rows)::value, 0xF, false);
+        v += __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+    };
+    using std::integral_constant;
+    step(integral_constant<int, 0x111>(), integral_constant<int, 0xF>());  // row_shr 1, 2, 4, 8
+    step(integral_constant<int, 0x112>(), integral_constant<int, 0xF>());
+    step(integral_constant<int, 0x114>(), integral_constant<int, 0xF>());
+    step(integral_constant<int, 0x118>(), integral_constant<int, 0xF>());
+    step(integral_constant<int, 0x142>(), integral_constant<int, 0xA>());  // row_bcast 15, 31
+    step(integral_constant<int, 0x143>(), integral_constant<int, 0xC>());
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, 63);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), 63);
+    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
 
+// log(s) for s > 0: float32's, and the first terms of log(1 + d), d = s exp(-that) - 1
+// some 1e-7.
+__device__ __forceinline__ double log_of(double s) {
+    const double y = (double)logf((float)s), d = s * exp_diff((float)-y, 0.0) - 1.0;
+    return y + d * (1.0 - 0.5 * d);
+}
+
+__device__ __forceinline__ uint64_t max_key(uint64_t a, uint64_t b) { return a > b ? a : b; }
+
+// A selection's LDS: the waves' best of each class, the list and its length.
 struct TopSh {
-    uint64_t floor;  // the want-th best of the threads' best
-    uint32_t count;  // candidates that reach it
+    uint64_t* tops;  // [waves * 64]
+    uint64_t* list;  // [room]
+    uint32_t* count;
+    int room;
 };
 
 // The best `want` (<= 64) of a workgroup's candidates.  mine: the thread's best
-// key (0: none); each(f): f(key) for every candidate of the thread; tops: LDS for
-// want keys a wave, list: for want times the most candidates that a thread has.
-// The want-th best of the threads' best is a floor that at least `want`
-// candidates reach (or all there are), and at most want threads hold any that
-// do, so a short list is left, whose members count those before them.
-// put(rank, key) is called once for each candidate taken.  Every step is a
-// comparison of distinct keys: the result does not depend on the order in which
-// the list was filled.
+// key (0: none); each(f): f(key) for every candidate of the thread.  The lanes
+// fall into 2^k >= want classes: the smallest of the classes' best is a floor that
+// at least `want` candidates reach, and seldom many more (want H(want) if they lie
+// anyhow), which are listed and count those before them.  Where more reach it
+// than the list holds, or a class is empty, the best key below the last one is
+// sought want times instead.  put(rank, key) is called once for each candidate
+// taken; returns how many there are.  Every step compares distinct keys: the
+// result does not depend on the order in which the list was filled.
 template <typename EACH, typename PUT>
-__device__ __forceinline__ void top_of(uint64_t mine, int want, TopSh& sh, uint64_t* tops, uint64_t* list, EACH each, PUT put) {
+__device__ __forceinline__ int top_of(uint64_t mine, int want, const TopSh& sh, EACH each, PUT put) {
     const int nt = blockDim.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nwave = nt >> 6;
-    if (want >= 64) {
-        tops[threadIdx.x] = mine;
-    } else {
-        uint32_t hi = (uint32_t)(mine >> 32);
-        const uint32_t lo = (uint32_t)mine;
-        uint64_t won = 0;  // lane r: the wave's r-th best
-        for (int r = 0; r < want; r++) {
-            const uint32_t top = wave_max_u32(hi);
-            if (!top) break;
-            uint64_t eq = __ballot(hi == top);
-            if (eq & (eq - 1)) {  // equal scores: the lowest place, the largest lower word
-                const uint32_t low = wave_max_u32(hi == top ? lo : 0u);
-                eq = __ballot(hi == top && lo == low);
-            }
-            const int src = __ffsll((unsigned long long)eq) - 1;
-            const uint32_t p = (uint32_t)__builtin_amdgcn_readlane((int)lo, src);
-            if (lane == r) won = ((uint64_t)top << 32) | p;
-            if (lane == src) hi = 0;
-        }
-        if (lane < want) tops[wave * want + lane] = won;
-    }
-    if (threadIdx.x == 0) {
-        sh.floor = 1;
-        sh.count = 0;
-    }
+    int classes = 1;
+    while (classes < want) classes *= 2;
+    uint64_t best = mine;
+    for (int k = 32; k >= classes; k >>= 1) best = max_key(best, __shfl_xor((unsigned long long)best, k));
+    if (lane < classes) sh.tops[wave * classes + lane] = best;
+    if (threadIdx.x == 0) *sh.count = 0;
     __syncthreads();
-    const int held = nwave * min(want, 64);
-    if ((int)threadIdx.x < held) {
-        const uint64_t k = tops[threadIdx.x];
-        int before = 0;
-        for (int j = 0; j < held; j++) before += tops[j] > k ? 1 : 0;
-        if (k && before == want - 1) sh.floor = k;
+    uint64_t floor = 0;
+    for (int w = 0; w < nwave; w++) floor = max_key(floor, sh.tops[w * classes + (lane & (classes - 1))]);
+    {
+        const uint32_t hi = ~wave_max_u32(~(uint32_t)(floor >> 32));
+        const uint32_t lo = ~wave_max_u32((uint32_t)(floor >> 32) == hi ? ~(uint32_t)floor : 0u);
+        floor = hi ? ((uint64_t)hi << 32) | lo : 1;
     }
-    __syncthreads();
-    const uint64_t floor = sh.floor;
     if (mine >= floor)
         each([&](uint64_t k) {
-            if (k >= floor) list[atomicAdd(&sh.count, 1u)] = k;
+            if (k >= floor) {
+                const uint32_t at = atomicAdd(sh.count, 1u);
+                if (at < (uint32_t)sh.room) sh.list[at] = k;
+            }
         });
     __syncthreads();
-    const int m = (int)sh.count;
-    for (int i = threadIdx.x; i < m; i += nt) {
-        const uint64_t k = list[i];
-        int before = 0;
-        for (int j = 0; j < m; j++) before += list[j] > k ? 1 : 0;
-        if (before < want) put(before, k);
+    const int m = (int)*sh.count;
+    if (m <= sh.room) {
+        for (int i = threadIdx.x; i < m; i += nt) {
+            const uint64_t k = sh.list[i];
+            int before = 0;
+#pragma unroll 4
+            for (int j = 0; j < m; j++) before += sh.list[j] > k ? 1 : 0;
+            if (before < want) put(before, k);
+        }
+        return min(m, want);
     }
+    uint64_t prev = ~0ull;
+    for (int r = 0; r < want; r++) {
+        best = 0;
+        each([&](uint64_t k) {
+            if (k < prev && k > best) best = k;
+        });
+        // the upper word's largest, then the lower word's among those
+        const uint32_t hi = wave_max_u32((uint32_t)(best >> 32));
+        const uint32_t lo = wave_max_u32((uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
+        if (lane == 0) sh.tops[wave] = ((uint64_t)hi << 32) | lo;
+        __syncthreads();
+        best = 0;
+        for (int w = 0; w < nwave; w++) best = max_key(best, sh.tops[w]);
+        __syncthreads();
+        if (!best) return r;
+        if (threadIdx.x == 0) put(r, best);
+        prev = best;
+    }
+    return want;
 }
 
 struct SelArgs {
@@ -178,63 +213,145 @@ __device__ __forceinline__ void put_rest(const SelArgs& a, int64_t g, int taken)
     }
 }
 
-// Few candidates (beams_in * n_outputs <= BS_ONE): one workgroup per group, the
-// logits read once into LDS.  parts waves share a beam.
+// Up to 1,024 outputs a beam: one workgroup per group, a wave for each R beams,
+// whose up to E * 64 outputs stay in registers from the load to the selection,
+// and no barrier before it.  What it costs is the chain of one wave: load, the
+// largest, E exponentials, the sum, a logarithm, the scores.  Measured, us, 8 x
+// 480 -> 8: one group 5.6 (the logits in LDS, between barriers: 10.4), 512 groups
+// 8.2 (13.6), 4,096 groups 35 (54); two beams a wave 7.0, 9.0, 33.
+template <typename T, int R, int E>
+__global__ void __launch_bounds__(1024) beam_small_kernel(SelArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint64_t small_sh[];  // tops, list: 64 a wave each
+    __shared__ uint32_t count;
+    const TopSh sh{small_sh, small_sh + blockDim.x, &count, (int)blockDim.x};
+    const int64_t g = blockIdx.x;
+    const int lane = threadIdx.x & 63, w0 = (threadIdx.x >> 6) * R;
+    const int n = live_of(a, g);
+    const T* x = (const T*)a.x + g * a.gs + w0 * a.bs + lane;
+    float v[R][E], m[R];
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int e = 0; e < E; e++) v[r][e] = w0 + r < a.win && e * 64 + lane < n ? up(x[r * a.bs + e * 64]) : -INFINITY;
+    float best = -INFINITY;
+    uint32_t at = 0;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        m[r] = -INFINITY;
+        bool nan = false;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            m[r] = fmaxf(m[r], v[r][e]);
+            nan |= v[r][e] != v[r][e];
+        }
+        m[r] = wave_max(nan ? INFINITY : m[r]);  // (a NaN spoils the beam as +infinity does)
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const bool fine = fabsf(m[r]) < INFINITY;
+        const double md = fine ? (double)m[r] : 0.0;
+        double s = 0.0;
+#pragma unroll
+        for (int e = 0; e < E; e++)
+            if (e * 64 < n) s += exp_diff(v[r][e], md);  // (the same branch for the whole wave)
+        s = wave_sum(s);
+        // (no finite logit, an infinite one or a NaN: no score of the beam is a number)
+        const double base = fine ? (double)a.score[g * a.win + w0 + r] - log_of(s) : (double)NAN;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            v[r][e] = (float)(((double)v[r][e] - md) + base);
+            if (v[r][e] > best) best = v[r][e], at = (uint32_t)(w0 + r) << 16 | (uint32_t)(e * 64 + lane);
+        }
+    }
+    // (a place in the key: beam and output in 16 bits each, in the same order)
+    const auto each = [&](auto f) {
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int e = 0; e < E; e++) f(make_key(score_bits(v[r][e]), (uint32_t)(w0 + r) << 16 | (uint32_t)(e * 64 + lane)));
+    };
+    const int taken = top_of(make_key(score_bits(best), at), a.wout, sh, each, [&](int r, uint64_t k) {
+        const uint32_t place = 0xFFFFFFFFu - (uint32_t)k;
+        const int64_t o = g * a.wout + r;
+        a.o_score[o] = bits_score((uint32_t)(k >> 32));
+        a.o_parent[o] = (int32_t)(place >> 16);
+        a.o_bucket[o] = (int32_t)(place & 0xFFFFu);
+    });
+    put_rest(a, g, taken);
+}
+
+// More (beams_in * n_outputs <= BS_ONE): one workgroup per group, the logits read
+// once into LDS.  parts waves share a beam.
 #define BS_ONE 8192
+#define BS_LIST 512
 template <typename T>
-__global__ void __launch_bounds__(1024) beam_select_kernel(SelArgs a, int parts) {
-    __shared__ TopSh sh;
+__global__ void __launch_bounds__(1024) beam_select_kernel(SelArgs a, int parts, uint32_t inv_v) {
+    __shared__ uint32_t count;
     __shared__ double sum[BS_MAX];   // [beam * parts + part]: parts > 1 only while beams * parts <= waves
     __shared__ float top[BS_MAX];
     __shared__ double base[BS_MAX];  // a beam's score - log(sum); NaN: none of its continuations counts
     __shared__ double largest[BS_MAX];  // its largest logit
-    extern __shared__ __attribute__((aligned(16))) float cand[];  // [win * v] logits, then scores; tops; list
+    extern __shared__ __attribute__((aligned(16))) uint64_t select_sh[];  // tops, list, [win * v] logits, then scores
+    const TopSh sh{select_sh, select_sh + blockDim.x, &count, BS_LIST};
+    float* cand = reinterpret_cast<float*>(select_sh + blockDim.x + BS_LIST);
     const int64_t g = blockIdx.x;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nwave = blockDim.x >> 6;
     const int n = live_of(a, g), rows = nwave / parts, part = wave % parts, first = wave / parts;
     const T* x = (const T*)a.x + g * a.gs;
     const int step = parts * 64, o0 = part * 64 + lane;
+    const int all = a.win * a.v;
+    for (int i0 = threadIdx.x; i0 < all; i0 += 16 * blockDim.x) {  // 16 loads of a thread under way at once
+        float v[16];
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const int i = i0 + j * blockDim.x;
+            const int w = a.v == 1 ? i : (int)__umulhi((uint32_t)i, inv_v), o = i - w * a.v;
+            v[j] = i < all && o < n ? up(x[(int64_t)w * a.bs + o]) : -INFINITY;
+        }
+#pragma unroll
+        for (int j = 0; j < 16; j++)
+            if (i0 + j * (int)blockDim.x < all) cand[i0 + j * blockDim.x] = v[j];
+    }
+    __syncthreads();
+    // eight of a beam's outputs a lane at a time, -infinity behind the live ones
+    const auto eight = [&](const float* c, int o, float (&v)[8]) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = o + j * step < n ? c[o + j * step] : -INFINITY;
+    };
     for (int w = first; w < a.win; w += rows) {
-        const T* p = x + (int64_t)w * a.bs;
-        float* c = cand + w * a.v;
         float m = -INFINITY;
         bool nan = false;
-        int o = o0;
-        for (; o + 7 * step < n; o += 8 * step) {
+        for (int o = o0; o - lane < n; o += 8 * step) {
             float v[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = up(p[o + j * step]);
+            eight(cand + w * a.v, o, v);
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                c[o + j * step] = v[j];
                 m = fmaxf(m, v[j]);
                 nan |= v[j] != v[j];
             }
         }
-#pragma unroll 4
-        for (; o < n; o += step) {
-            const float v = up(p[o]);
-            c[o] = v;
-            m = fmaxf(m, v);
-            nan |= v != v;
-        }
-        m = wave_max(m);
-        const bool spoilt = __ballot(nan) != 0;  // (a NaN spoils the beam as +infinity does)
-        if (lane == 0) top[w * parts + part] = spoilt ? INFINITY : m;
+        m = wave_max(nan ? INFINITY : m);  // (a NaN spoils the beam as +infinity does)
+        if (lane == 0) top[w * parts + part] = m;
     }
     __syncthreads();
     for (int w = first; w < a.win; w += rows) {
         float m = top[w * parts];
         for (int k = 1; k < parts; k++) m = fmaxf(m, top[w * parts + k]);
-        const float* c = cand + w * a.v;
         const double md = (double)m;
-        double s = 0.0;
-        if (fabsf(m) < INFINITY) {
-#pragma unroll 4
-            for (int o = o0; o < n; o += step) s += exp_diff(c[o], md);
-        }
-        s = wave_sum(s);
-        if (lane == 0) sum[w * parts + part] = s;
+        double s[2] = {0.0, 0.0};
+        if (fabsf(m) < INFINITY)
+            for (int o = o0; o - lane < n; o += 8 * step) {
+                float v[8];
+                eight(cand + w * a.v, o, v);
+#pragma unroll
+                for (int j = 0; j < 8; j += 2)
+                    if (o - lane + j * step < n) {  // (the same for the whole wave)
+                        s[0] += exp_diff(v[j], md);
+                        s[1] += exp_diff(v[j + 1], md);
+                    }
+            }
+        s[0] = wave_sum(s[0] + s[1]);
+        if (lane == 0) sum[w * parts + part] = s[0];
     }
     __syncthreads();
     if ((int)threadIdx.x < a.win) {
@@ -247,7 +364,7 @@ __global__ void __launch_bounds__(1024) beam_select_kernel(SelArgs a, int parts)
         }
         largest[w] = (double)m;
         // (no finite logit, an infinite one or a NaN: no score of the beam is a number)
-        base[w] = fabsf(m) < INFINITY ? (double)a.score[g * a.win + w] - log(s) : (double)NAN;
+        base[w] = fabsf(m) < INFINITY ? (double)a.score[g * a.win + w] - log_of(s) : (double)NAN;
     }
     __syncthreads();
     float best = -INFINITY;
@@ -255,23 +372,30 @@ __global__ void __launch_bounds__(1024) beam_select_kernel(SelArgs a, int parts)
     for (int w = first; w < a.win; w += rows) {
         const double b = base[w], m = largest[w];
         float* c = cand + w * a.v;
-#pragma unroll 4
-        for (int o = o0; o < n; o += step) {
-            const float v = (float)(((double)c[o] - m) + b);
-            c[o] = v;
-            if (v > best) best = v, at = (uint32_t)(w * a.v + o);
+        for (int o = o0; o - lane < n; o += 8 * step) {
+            float v[8];
+            eight(c, o, v);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (o + j * step < n) {
+                    v[j] = (float)(((double)v[j] - m) + b);
+                    c[o + j * step] = v[j];
+                    if (v[j] > best) best = v[j], at = (uint32_t)(w * a.v + o + j * step);
+                }
         }
     }
-    const int all = a.win * a.v;
-    uint64_t* tops = reinterpret_cast<uint64_t*>(cand + ((all + 1) & ~1));
     const auto each = [&](auto f) {
         for (int w = first; w < a.win; w += rows)
-            for (int o = o0; o < n; o += step) f(make_key(score_bits(cand[w * a.v + o]), (uint32_t)(w * a.v + o)));
+            for (int o = o0; o - lane < n; o += 8 * step) {
+                float v[8];
+                eight(cand + w * a.v, o, v);
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (v[j] > -INFINITY) f(make_key(score_bits(v[j]), (uint32_t)(w * a.v + o + j * step)));
+            }
     };
-    top_of(make_key(score_bits(best), at), a.wout, sh, tops, tops + nwave * a.wout, each,
-           [&](int r, uint64_t k) { put_key(a, g, r, k); });
-    __syncthreads();
-    put_rest(a, g, min((int)sh.count, a.wout));
+    const int taken = top_of(make_key(score_bits(best), at), a.wout, sh, each, [&](int r, uint64_t k) { put_key(a, g, r, k); });
+    put_rest(a, g, taken);
 }
 
 // Many candidates: chunks of BS_CHUNK of a beam's outputs, three launches.
@@ -323,8 +447,9 @@ __global__ void __launch_bounds__(256) beam_sums_kernel(SelArgs a, SelWork k, in
 
 template <typename T>
 __global__ void __launch_bounds__(256) beam_chunk_kernel(SelArgs a, SelWork k, int64_t row0) {
-    __shared__ TopSh sh;
-    __shared__ uint64_t tops[BS_MAX * 4], list[BS_MAX * (BS_CHUNK / 256)];
+    __shared__ uint64_t tops[4 * 64], list[1024];
+    __shared__ uint32_t count;
+    const TopSh sh{tops, list, &count, 1024};
     __shared__ float tm[4];
     __shared__ double ts[4];
     const int64_t row = row0 + blockIdx.y, g = row / a.win;
@@ -354,7 +479,7 @@ __global__ void __launch_bounds__(256) beam_chunk_kernel(SelArgs a, SelWork k, i
     if (lane == 0) ts[wave] = s;
     __syncthreads();
     s = (ts[0] + ts[1]) + (ts[2] + ts[3]);
-    const double base = fabsf(m) < INFINITY ? (double)a.score[row] - log(s) : (double)NAN;
+    const double base = fabsf(m) < INFINITY ? (double)a.score[row] - log_of(s) : (double)NAN;
     float best = -INFINITY;
     uint32_t at = 0;
     const uint32_t place0 = (uint32_t)(w * (int64_t)a.v + o0);
@@ -368,55 +493,24 @@ __global__ void __launch_bounds__(256) beam_chunk_kernel(SelArgs a, SelWork k, i
 #pragma unroll
         for (int j = 0; j < BS_CHUNK / 256; j++) f(make_key(score_bits(v[j]), place0 + j * 256 + threadIdx.x));
     };
-    top_of(make_key(score_bits(best), at), a.wout, sh, tops, list, each, [&](int r, uint64_t key) { keys[r] = key; });
-    __syncthreads();
-    for (int r = (int)sh.count + (int)threadIdx.x; r < a.wout; r += 256) keys[r] = 0;
+    const int taken = top_of(make_key(score_bits(best), at), a.wout, sh, each, [&](int r, uint64_t key) { keys[r] = key; });
+    for (int r = taken + (int)threadIdx.x; r < a.wout; r += 256) keys[r] = 0;
 }
 
-// The chunks' best of one group: the best of them.  A thread has at most `held`
-// keys (list: wout * held in dynamic LDS, behind the waves' tops).
+// The chunks' best of one group: the best of them.
 __global__ void __launch_bounds__(1024) beam_merge_kernel(SelArgs a, SelWork k) {
-    __shared__ TopSh sh;
-    extern __shared__ __attribute__((aligned(16))) uint64_t lds[];
+    __shared__ uint64_t tops[16 * 64], list[1024];
+    __shared__ uint32_t count;
+    const TopSh sh{tops, list, &count, 1024};
     const int64_t g = blockIdx.x, n = (int64_t)a.win * k.chunks * a.wout;
     const uint64_t* keys = k.keys + g * n;
     uint64_t best = 0;
 #pragma unroll 4
-    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) best = keys[i] > best ? keys[i] : best;
+    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) best = max_key(best, keys[i]);
     const auto each = [&](auto f) {
         for (int64_t i = threadIdx.x; i < n; i += blockDim.x) f(keys[i]);
     };
-    top_of(best, a.wout, sh, lds, lds + (blockDim.x >> 6) * a.wout, each, [&](int r, uint64_t key) { put_key(a, g, r, key); });
-    __syncthreads();
-    put_rest(a, g, min((int)sh.count, a.wout));
-}
-
-// The same for so many chunks that such a list does not fit: the best key below
-// the last one taken, wout times.
-__global__ void __launch_bounds__(1024) beam_merge_many_kernel(SelArgs a, SelWork k) {
-    __shared__ uint64_t red[16];
-    const int64_t g = blockIdx.x, n = (int64_t)a.win * k.chunks * a.wout;
-    const uint64_t* keys = k.keys + g * n;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint64_t prev = ~0ull;
-    int r = 0;
-    for (; r < a.wout; r++) {
-        uint64_t best = 0;
-        for (int64_t i = threadIdx.x; i < n; i += 1024)
-            if (keys[i] < prev && keys[i] > best) best = keys[i];
-        // the upper word's largest, then the lower word's among those
-        const uint32_t hi = wave_max_u32((uint32_t)(best >> 32));
-        const uint32_t lo = wave_max_u32((uint32_t)(best >> 32) == hi ? (uint32_t)best : 0u);
-        if (lane == 0) red[wave] = ((uint64_t)hi << 32) | lo;
-        __syncthreads();
-        best = 0;
-        for (int j = 0; j < 16; j++) best = red[j] > best ? red[j] : best;
-        __syncthreads();
-        if (!(best >> 32)) break;
-        if (threadIdx.x == 0) put_key(a, g, r, best);
-        prev = best;
-    }
-    put_rest(a, g, r);
+    put_rest(a, g, top_of(best, a.wout, sh, each, [&](int r, uint64_t key) { put_key(a, g, r, key); }));
 }
 
 // ------------------------------------------------------------------- rows
@@ -579,10 +673,15 @@ int rows_move(const RowMoves& m, const int32_t* idx, int64_t n_rows, int32_t bea
 
 extern "C" {
 
+// a beam's outputs fit a wave's registers, and 16 waves the beams
+static bool sel_small(int32_t win, int32_t v) { return v <= 1024 && win <= (v <= 256 ? 64 : v <= 512 ? 32 : 16); }
+
 static int sel_chunks(int32_t v) { return (v + BS_CHUNK - 1) / BS_CHUNK; }
 
 size_t htm_beam_work_bytes(int32_t groups, int32_t win, int32_t wout, int32_t v) {
-    if (groups < 1 || win < 1 || win > BS_MAX || wout < 1 || wout > BS_MAX || v < 1 || (int64_t)win * v <= BS_ONE) return 0;
+    if (groups < 1 || win < 1 || win > BS_MAX || wout < 1 || wout > BS_MAX || v < 1 || sel_small(win, v) ||
+        (int64_t)win * v <= BS_ONE)
+        return 0;
     return (size_t)groups * win * sel_chunks(v) * (8 + 8 + 8 * (size_t)wout);
 }
 
@@ -591,13 +690,25 @@ size_t htm_beam_work_bytes(int32_t groups, int32_t win, int32_t wout, int32_t v)
 template <typename T>
 static int select_launch(const SelArgs& a, int32_t groups, void* work, hipStream_t st) {
     const int64_t all = (int64_t)a.win * a.v;
+    if (sel_small(a.win, a.v)) {
+        const int each = (a.win + 15) / 16, waves = each > 2 ? (a.win + 3) / 4 : (a.win + each - 1) / each;
+        const auto small = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(groups), dim3(waves * 64), waves * 64 * 16, st, a);
+        };
+        if (each > 2) small(beam_small_kernel<T, 4, 4>);
+        else if (each == 2) a.v <= 256 ? small(beam_small_kernel<T, 2, 4>) : small(beam_small_kernel<T, 2, 8>);
+        else if (a.v <= 256) small(beam_small_kernel<T, 1, 4>);
+        else if (a.v <= 512) small(beam_small_kernel<T, 1, 8>);
+        else small(beam_small_kernel<T, 1, 16>);
+        return HTM_OK;
+    }
     if (all <= BS_ONE) {
-        // up to 16 candidates a thread; a few groups alone get 1,024 threads
-        const int nt = all > 4096 || (groups < 256 && all > 1024) ? 1024 : 256;
+        // (100 groups of 4 x 2,000: 256 threads 15.2 us, 512 12.7, 1,024 13.3; 2,000 groups: 39, 42, 90)
+        const int nt = groups < 512 ? 512 : 256;
         int parts = 1;
         while (parts * 2 * a.win <= nt / 64) parts *= 2;
-        const size_t lds = ((size_t)(all + 1) / 2 * 2) * 4 + (size_t)a.wout * (nt / 64 + (all + nt - 1) / nt) * 8;
-        hipLaunchKernelGGL(beam_select_kernel<T>, dim3(groups), dim3(nt), lds, st, a, parts);
+        const size_t lds = (size_t)(nt + BS_LIST) * sizeof(uint64_t) + (size_t)all * sizeof(float);
+        hipLaunchKernelGGL(beam_select_kernel<T>, dim3(groups), dim3(nt), lds, st, a, parts, 0xFFFFFFFFu / (uint32_t)a.v + 1u);
         return HTM_OK;
     }
     SelWork k;
@@ -612,10 +723,7 @@ static int select_launch(const SelArgs& a, int32_t groups, void* work, hipStream
         hipLaunchKernelGGL(beam_chunk_kernel<T>, grid, dim3(256), 0, st, a, k, r0);
     }
     const int64_t keys = (int64_t)a.win * k.chunks * a.wout;
-    const int nt = keys > 2048 ? 1024 : 256;
-    const int64_t lds = 8 * (int64_t)a.wout * (nt / 64 + (keys + nt - 1) / nt);
-    if (lds <= 60 * 1024) hipLaunchKernelGGL(beam_merge_kernel, dim3(groups), dim3(nt), (size_t)lds, st, a, k);
-    else hipLaunchKernelGGL(beam_merge_many_kernel, dim3(groups), dim3(1024), 0, st, a, k);
+    hipLaunchKernelGGL(beam_merge_kernel, dim3(groups), dim3(keys > 2048 ? 1024 : 256), 0, st, a, k);
     return HTM_OK;
 }
 

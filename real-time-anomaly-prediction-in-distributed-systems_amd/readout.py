@@ -175,7 +175,7 @@ class Readout4:
         import torch
         shape = (n, self.n_heads, self.n_outputs)
         if out is None:
-            return torch.empty(shape, dtype=torch.float32, device=self.device)
+            return self.records.new_empty(shape, dtype=torch.float32)
         if not isinstance(out, torch.Tensor) or out.dtype != torch.float32 or out.device != self.device or \
                 out.shape != shape or not out.is_contiguous():
             raise ValueError("out must be a contiguous float32 tensor %s on %s" % (shape, self.device))
