@@ -358,20 +358,26 @@ __global__ void __launch_bounds__(Q4_NT) q4_softmax_kernel(Q4Dims d, const int32
 #define MV_NT 256
 #define MV_HB 16     // outputs of a half block
 
+// (a & mask) | bits as one instruction: its operands allow one constant, so the
+// other has to be kept in a register, which the compiler does not do by itself.
+__device__ __forceinline__ uint32_t in_vgpr(uint32_t c) {
+    asm("" : "+v"(c));
+    return c;
+}
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) { return (a & mask) | bits; }
+
 template <int NX>
 struct MvAcc {
     float v[NX][MV_HB];
-    __device__ __forceinline__ void add(uint2 c, float s, const float* x) {
+    __device__ __forceinline__ void add(uint2 c, float s, const float* x, uint32_t e1032, uint32_t e72) {
         const half2_t k0 = {(_Float16)1032.0f, (_Float16)1032.0f}, k1 = {(_Float16)72.0f, (_Float16)72.0f};
         const uint32_t w[2] = {c.x, c.y};
         const float m = NX == 1 ? s * x[0] : s;
 #pragma unroll
         for (int k = 0; k < 2; k++) {
             const uint32_t h = w[k] >> 8;
-            const half2_t q[4] = {as_half2((w[k] & 0x000F000Fu) | 0x64006400u) - k0,
-                                  as_half2((w[k] & 0x00F000F0u) | 0x54005400u) - k1,
-                                  as_half2((h & 0x000F000Fu) | 0x64006400u) - k0,
-                                  as_half2((h & 0x00F000F0u) | 0x54005400u) - k1};
+            const half2_t q[4] = {as_half2(and_or(w[k], 0x000F000Fu, e1032)) - k0, as_half2(and_or(w[k], 0x00F000F0u, e72)) - k1,
+                                  as_half2(and_or(h, 0x000F000Fu, e1032)) - k0, as_half2(and_or(h, 0x00F000F0u, e72)) - k1};
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const float n = (float)(j < 4 ? q[j & 3].x : q[j & 3].y);
@@ -388,7 +394,7 @@ struct MvAcc {
 };
 
 template <typename T, int NX>
-__global__ void __launch_bounds__(MV_NT, NX == 8 ? 2 : NX == 4 ? 3 : 4)
+__global__ void __launch_bounds__(MV_NT, NX == 4 ? 3 : 4)
     q4_matvec_kernel(Q4Dims d, const uint8_t* __restrict__ rec, const T* __restrict__ x, int64_t xs, int per, int y0,
                      int passes, int cb, int chunks, int range, float* __restrict__ out, int64_t split_stride) {
     constexpr int KPT = 8 / NX, TILE = MV_NT * KPT;  // inputs of a thread and of a tile
@@ -396,7 +402,7 @@ __global__ void __launch_bounds__(MV_NT, NX == 8 ? 2 : NX == 4 ? 3 : 4)
     __shared__ __attribute__((aligned(16))) float xv[TILE][NX];
     __shared__ uint32_t wsum[MV_NT / 64];
     __shared__ float sm[MV_HB][MV_NT + 1];
-    const int chunk = blockIdx.x % chunks, split = blockIdx.x / chunks;
+    const int splits = gridDim.x / chunks, split = blockIdx.x % splits, chunk = blockIdx.x / splits;
     const int y = y0 + blockIdx.y, model = y / passes, q0 = (y - model * passes) * NX;
     const int nx = min(NX, per - q0);
     const int64_t row = (int64_t)model * per + q0;
@@ -409,6 +415,7 @@ __global__ void __launch_bounds__(MV_NT, NX == 8 ? 2 : NX == 4 ? 3 : 4)
     const uint8_t* sbase = base + d.scales + 2 * (h * d.ngrp + (hb - h * d.nblk * 2) * MV_HB / d.group);
     const uint32_t pitch64 = d.pitch / 64;
     const int k0 = split * range, k1 = min(d.ni, k0 + range);
+    const uint32_t e1032 = in_vgpr(0x64006400u), e72 = in_vgpr(0x54005400u);
     MvAcc<NX> a;
 #pragma unroll
     for (int r = 0; r < NX; r++)
@@ -474,7 +481,7 @@ __global__ void __launch_bounds__(MV_NT, NX == 8 ? 2 : NX == 4 ? 3 : 4)
                     float xr[NX];
 #pragma unroll
                     for (int r = 0; r < NX; r++) xr[r] = xv[i + u][r];
-                    a.add(c[u], bf16_up(s[u]), xr);
+                    a.add(c[u], bf16_up(s[u]), xr, e1032, e72);
                 }
                 i += U;
             };
@@ -502,6 +509,176 @@ __global__ void __launch_bounds__(MV_NT, NX == 8 ? 2 : NX == 4 ? 3 : 4)
             const int b = b0 + (k >> 4), hh = b / (d.nblk * 2), j = (b - hh * d.nblk * 2) * MV_HB + (k & 15);
             if (j < d.no) o[(int64_t)r * d.nh * d.no + hh * d.no + j] = y;
         }
+    }
+}
+
+// Several rows at once, by matrix instructions.  v_mfma_f32_16x16x32_bf16 takes 16
+// rows' numbers for 32 inputs (A) and those inputs' weights of 16 outputs (B).  A
+// weight scale * (code - 8) has 8 + 4 bits, too many for a bfloat16: the scale's
+// upper and lower four bits make two bfloat16 products that are exact, and a
+// number takes one (bfloat16), two (float16) or three (float32) bfloat16 parts,
+// so that every product in the sum is exact and only float32 sums round, as in the
+// kernel above, while a weight costs some 4.4 instructions for all 16 rows
+// instead of 3 and one for each row.
+//
+// One workgroup per (16 rows of one matrix, 16 half blocks, range of inputs).  The
+// tile's inputs are listed as above, with their numbers' parts in LDS; its waves
+// take 32 of the list in turn.  Lane l loads inputs (l / 16) * 8 .. + 7 of half
+// block l % 16, which are B for each of the half block's 16 outputs: 16 sums of
+// [16 rows x 16 half blocks], one for each output of a half block.
+#define MM_NT 256
+#define MM_ROWS 16
+#define MM_TILE 256
+#define MM_PITCH (MM_TILE + 8)   // bfloat16 of a row in LDS: 16-byte reads of 16 rows fall on different banks
+#define MM_COLS 272              // floats of a row in the join: 16 x 17
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T> struct MmParts { static constexpr int n = 3; };
+template <> struct MmParts<__half> { static constexpr int n = 2; };
+template <> struct MmParts<__hip_bfloat16> { static constexpr int n = 1; };
+
+template <typename T>
+__global__ void __launch_bounds__(MM_NT, 2)
+    q4_mfma_kernel(Q4Dims d, const uint8_t* __restrict__ rec, const T* __restrict__ x, int64_t xs, int per, int y0,
+                   int passes, int tiles, int range, float* __restrict__ out, int64_t split_stride) {
+    constexpr int P = MmParts<T>::n;
+    extern __shared__ __attribute__((aligned(16))) uint8_t mm_sh[];
+    __shared__ uint32_t list[MM_TILE + 32];
+    __shared__ uint32_t wsum[MM_NT / 64];
+    uint16_t* xa = reinterpret_cast<uint16_t*>(mm_sh);  // [P][MM_ROWS][MM_PITCH]
+    const int splits = gridDim.x / tiles, split = blockIdx.x % splits, tile = blockIdx.x / splits;
+    const int y = y0 + blockIdx.y, model = y / passes, q0 = (y - model * passes) * MM_ROWS;
+    const int nx = min(MM_ROWS, per - q0);
+    const int64_t row = (int64_t)model * per + q0;
+    const int halves = d.nh * d.nblk * 2;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int hb = min(tile * 16 + (lane & 15), halves - 1);  // (behind the last: computed again and not written)
+    const uint8_t* base = rec + (int64_t)model * d.ni * d.pitch;
+    const int h = hb / (d.nblk * 2);
+    const uint8_t* cbase = base + hb * 8;
+    const uint8_t* sbase = base + d.scales + 2 * (h * d.ngrp + (hb - h * d.nblk * 2) * MV_HB / d.group);
+    const uint32_t pitch64 = d.pitch / 64;
+    const int k0 = split * range, k1 = min(d.ni, k0 + range);
+    const uint32_t e1032 = in_vgpr(0x64006400u), e72 = in_vgpr(0x54005400u);
+    f32x4 acc[MV_HB];
+#pragma unroll
+    for (int j = 0; j < MV_HB; j++) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float mine[MM_ROWS];
+    auto fetch = [&](int t0) {
+        const int k = t0 + (int)threadIdx.x;
+#pragma unroll
+        for (int r = 0; r < MM_ROWS; r++) mine[r] = k < k1 && r < nx ? x_up(x[(row + r) * xs + k]) : 0.0f;
+    };
+    fetch(k0);
+    for (int t0 = k0; t0 < k1; t0 += MM_TILE) {
+        bool some = false;
+#pragma unroll
+        for (int r = 0; r < MM_ROWS; r++) some |= mine[r] != 0.0f;
+        const uint64_t bal = __ballot(some);
+        if (lane == 0) wsum[wave] = (uint32_t)__popcll(bal);
+        __syncthreads();
+        uint32_t at = (uint32_t)__popcll(bal & ((1ull << lane) - 1ull)), m = 0;
+#pragma unroll
+        for (int k = 0; k < MM_NT / 64; k++) {
+            if (k < wave) at += wsum[k];
+            m += wsum[k];
+        }
+        // up to a multiple of 32 behind the list: the tile's first input, times zero
+        const uint32_t pad = (32u - (m & 31u)) & 31u;
+        const bool fill = threadIdx.x < pad;
+        if (some) list[at] = (uint32_t)(t0 + (int)threadIdx.x) * pitch64;
+        if (fill) list[m + threadIdx.x] = (uint32_t)t0 * pitch64;
+#pragma unroll
+        for (int r = 0; r < MM_ROWS; r++) {
+            float v = mine[r];
+#pragma unroll
+            for (int p = 0; p < P; p++) {
+                uint32_t u = __float_as_uint(v) & 0xFFFF0000u;
+                if (v != v) u = 0x7FC00000u;
+                // (what is left of an infinity or a NaN is not a part)
+                v = fabsf(v) < INFINITY ? v - __uint_as_float(u) : 0.0f;
+                if (some) xa[(p * MM_ROWS + r) * MM_PITCH + at] = (uint16_t)(u >> 16);
+                if (fill) xa[(p * MM_ROWS + r) * MM_PITCH + m + threadIdx.x] = 0;
+            }
+        }
+        __syncthreads();
+        fetch(t0 + MM_TILE);  // (the next tile's numbers meanwhile)
+        for (int q = wave * 32; q < (int)m; q += MM_NT / 2) {
+            const int q8 = q + (lane >> 4) * 8;
+            uint2 c[8];
+            uint32_t sc[8];
+#pragma unroll
+            for (int r = 0; r < 8; r++) {
+                const uint64_t o = (uint64_t)list[q8 + r] << 6;
+                c[r] = *reinterpret_cast<const uint2*>(cbase + o);
+                sc[r] = *reinterpret_cast<const uint16_t*>(sbase + o);
+            }
+            bf16x8 a[P];
+#pragma unroll
+            for (int p = 0; p < P; p++)
+                a[p] = *reinterpret_cast<const bf16x8*>(xa + (p * MM_ROWS + (lane & 15)) * MM_PITCH + q8);
+            __builtin_amdgcn_sched_barrier(0);  // (every load is under way before the first is waited for)
+            float hi[8], lo[8];
+#pragma unroll
+            for (int r = 0; r < 8; r++) {
+                hi[r] = bf16_up(sc[r] & 0xFFF0u);
+                lo[r] = bf16_up(sc[r]) - hi[r];
+            }
+#pragma unroll
+            for (int g = 0; g < 4; g++) {  // four outputs: half a word of each input's codes
+                uint32_t w[4];
+#pragma unroll
+                for (int p = 0; p < 4; p++)
+                    w[p] = __builtin_amdgcn_perm(g < 2 ? c[2 * p + 1].x : c[2 * p + 1].y, g < 2 ? c[2 * p].x : c[2 * p].y,
+                                                 g & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+                for (int n = 0; n < 4; n++) {
+                    const half2_t bias = n & 1 ? half2_t{(_Float16)72.0f, (_Float16)72.0f}
+                                               : half2_t{(_Float16)1032.0f, (_Float16)1032.0f};
+                    u32x4 bh, bl;
+#pragma unroll
+                    for (int p = 0; p < 4; p++) {
+                        const uint32_t u = n < 2 ? w[p] : w[p] >> 8;
+                        const half2_t q2 = as_half2(n & 1 ? and_or(u, 0x00F000F0u, e72) : and_or(u, 0x000F000Fu, e1032)) - bias;
+                        const float a0 = __builtin_fmaf((float)q2.x, hi[2 * p], 0.0f);
+                        const float a1 = __builtin_fmaf((float)q2.y, hi[2 * p + 1], 0.0f);
+                        const float b0 = __builtin_fmaf((float)q2.x, lo[2 * p], 0.0f);
+                        const float b1 = __builtin_fmaf((float)q2.y, lo[2 * p + 1], 0.0f);
+                        bh[p] = __builtin_amdgcn_perm(__float_as_uint(a1), __float_as_uint(a0), 0x07060302u);
+                        bl[p] = __builtin_amdgcn_perm(__float_as_uint(b1), __float_as_uint(b0), 0x07060302u);
+                    }
+                    const int j = g * 4 + n;
+#pragma unroll
+                    for (int p = 0; p < P; p++) {
+                        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[p], __builtin_bit_cast(bf16x8, bl), acc[j], 0, 0, 0);
+                        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[p], __builtin_bit_cast(bf16x8, bh), acc[j], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    }
+    // the four waves' sums
+    __syncthreads();
+    float* jn = reinterpret_cast<float*>(mm_sh);  // [wave][row][output of 16][half block of 16 + 1]
+#pragma unroll
+    for (int j = 0; j < MV_HB; j++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = (lane >> 4) * 4 + i;
+            if (r < nx) jn[(wave * nx + r) * MM_COLS + j * 17 + (lane & 15)] = acc[j][i];
+        }
+    __syncthreads();
+    const int b = tile * 16 + (int)threadIdx.x / 16, j = threadIdx.x & 15;
+    const int hh = b / (d.nblk * 2), col = (b - hh * d.nblk * 2) * MV_HB + j;
+    if (b >= halves || col >= d.no) return;
+    float* o = out + split * split_stride + row * d.nh * d.no + hh * d.no + col;
+    for (int r = 0; r < nx; r++) {
+        const float* p = jn + r * MM_COLS + j * 17 + threadIdx.x / 16;
+        const int w = nx * MM_COLS;
+        o[(int64_t)r * d.nh * d.no] = (p[0] + p[w]) + (p[2 * w] + p[3 * w]);
     }
 }
 
@@ -575,29 +752,54 @@ static int q4_bitmap(const htm_q4_shape* s, const void* rec, const uint32_t* pat
 
 #define Q4_GRID_Y 65535  // rows of one launch
 
-// How a product is shared out: NX rows at a time, runs of half blocks and ranges
-// of inputs, some 512 workgroups in all.  Measured, us (runs x ranges, both
-// launches; rows, inputs, outputs):
-//   8, 24,576, 7 x 480: 7 x 73 44, 7 x 36 50, 14 x 36 47, 4 x 64 58
-//   8, 24,576, 480: 2 x 128 20, 1 x 128 23, 1 x 64 30
-//   12, 4,000, 7 x 480: 14 x 16 22, 7 x 32 23, 7 x 8 38, 210 x 1 57
-//   8, 1,000, 7 x 500: 14 x 4 17, 7 x 8 18, 112 x 1 26
-//   1, 4,000, 480: 2 x 16 9.3, 30 x 1 12.5
-// In one launch while a tile holds the inputs (1, 300, 1,000: 16 x 1 5.7, 4 x 4
-// 7.1; 1, 2,048 with 6 % not zero, 480: 10 x 1 5.9, 2 x 8 7.0).
+// More than 64 KiB of dynamic LDS: allowed once per kernel and device.
+static int q4_raise_lds(const void* kernel, size_t lds, std::atomic<uint64_t>& raised) {
+    if (lds <= 65536) return HTM_OK;
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return htm_fail(HTM_E_HIP, "q4: no current device");
+    const uint64_t bit = 1ull << (dev & 63);
+    if (dev < 64 && (raised.load() & bit)) return HTM_OK;
+    if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 150 * 1024) != hipSuccess)
+        return htm_fail(HTM_E_HIP, "q4: cannot raise the dynamic LDS limit to %zu B", lds);
+    if (dev < 64) raised.fetch_or(bit);
+    return HTM_OK;
+}
+
+// How a product is shared out: rows at a time, runs of half blocks and ranges of
+// inputs, some 512 workgroups in all.  Measured, us, both launches:
+//   rows, inputs, outputs          4 rows a pass   8 rows    matrix instructions
+//   1, 24,576, 7 x 480             22 (one row)              35
+//   4, 24,576, 7 x 480             30                        36
+//   8, 24,576, 7 x 480                             44        36 (bfloat16 34)
+//   16, 24,576, 7 x 480                            69        38
+//   8, 24,576, 480                                 18        15
+//   12, 4,000, 7 x 480                             21        16
+//   8, 1,000, 7 x 500                              16        12 (ranges of 256: 14)
+// and for the first two columns, runs x ranges: 8, 24,576, 7 x 480: 7 x 73 44, 7 x
+// 36 50, 4 x 64 58; 1, 4,000, 480: 2 x 16 9.3, 30 x 1 12.5.  In one launch while a
+// tile holds the inputs: 1, 300, 1,000: 16 x 1 5.7, 4 x 4 7.1; 1, 2,048 with 6 %
+// not zero, 480: 10 x 1 5.9, 2 x 8 7.0.
 struct MvPlan {
+    bool mfma;
     int nx, passes, cb, chunks, splits, range;
 };
 
 static MvPlan mv_plan(const Q4Dims& d, int per) {
     MvPlan p;
-    p.nx = per >= 5 ? 8 : per >= 3 ? 4 : per;
+    p.mfma = per >= 5;
+    p.nx = p.mfma ? MM_ROWS : per >= 3 ? 4 : per;
     p.passes = (per + p.nx - 1) / p.nx;
     const int64_t y = (int64_t)d.nm * p.passes;
     const int halves = d.nh * d.nblk * 2;
     p.splits = 1;
     const int64_t few = 512;
-    if ((d.ni <= 256 || (per == 1 && d.ni <= 2048)) && (halves + 3) / 4 * y <= few) {
+    if (p.mfma) {
+        const int64_t most = (d.ni + (d.ni <= 2048 ? 127 : 255)) / (d.ni <= 2048 ? 128 : 256);
+        p.chunks = (halves + 15) / 16;
+        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(few / (p.chunks * y), most));
+        // (a range's workgroups on one XCD: their pieces of a record share its lines)
+        if (p.splits >= 8) p.splits = p.splits / 8 * 8;
+    } else if ((d.ni <= 256 || (per == 1 && d.ni <= 2048)) && (halves + 3) / 4 * y <= few) {
         p.chunks = (halves + 3) / 4;
     } else {
         const int64_t most = (d.ni + 255) / 256;
@@ -613,32 +815,27 @@ static MvPlan mv_plan(const Q4Dims& d, int per) {
 }
 
 template <typename T>
-static void mv_launch(const MvPlan& p, const Q4Dims& d, const void* rec, const void* x, int64_t xs, int per, float* out,
+static int mv_launch(const MvPlan& p, const Q4Dims& d, const void* rec, const void* x, int64_t xs, int per, float* out,
                       int64_t stride, hipStream_t st) {
     const int64_t all = (int64_t)d.nm * p.passes;
+    const size_t lds = std::max<size_t>((size_t)MmParts<T>::n * MM_ROWS * MM_PITCH * 2,
+                                        (size_t)4 * std::min(per, MM_ROWS) * MM_COLS * sizeof(float));
+    static std::atomic<uint64_t> raised{0};
+    if (p.mfma)
+        if (int r = q4_raise_lds((const void*)q4_mfma_kernel<T>, lds, raised)) return r;
     for (int64_t y0 = 0; y0 < all; y0 += Q4_GRID_Y) {
         const dim3 grid(p.chunks * p.splits, (uint32_t)std::min<int64_t>(all - y0, Q4_GRID_Y));
         const auto go = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, grid, dim3(MV_NT), 0, st, d, (const uint8_t*)rec, (const T*)x, xs, per, (int)y0, p.passes,
                                p.cb, p.chunks, p.range, out, stride);
         };
-        if (p.nx == 1) go(q4_matvec_kernel<T, 1>);
+        if (p.mfma)
+            hipLaunchKernelGGL(q4_mfma_kernel<T>, grid, dim3(MM_NT), lds, st, d, (const uint8_t*)rec, (const T*)x, xs, per,
+                               (int)y0, p.passes, p.chunks, p.range, out, stride);
+        else if (p.nx == 1) go(q4_matvec_kernel<T, 1>);
         else if (p.nx == 2) go(q4_matvec_kernel<T, 2>);
-        else if (p.nx == 4) go(q4_matvec_kernel<T, 4>);
-        else go(q4_matvec_kernel<T, 8>);
+        else go(q4_matvec_kernel<T, 4>);
     }
-}
-
-// More than 64 KiB of dynamic LDS: allowed once per kernel and device.
-static int q4_raise_lds(const void* kernel, size_t lds, std::atomic<uint64_t>& raised) {
-    if (lds <= 65536) return HTM_OK;
-    int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess) return htm_fail(HTM_E_HIP, "q4: no current device");
-    const uint64_t bit = 1ull << (dev & 63);
-    if (dev < 64 && (raised.load() & bit)) return HTM_OK;
-    if (hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 150 * 1024) != hipSuccess)
-        return htm_fail(HTM_E_HIP, "q4: cannot raise the dynamic LDS limit to %zu B", lds);
-    if (dev < 64) raised.fetch_or(bit);
     return HTM_OK;
 }
 
@@ -731,9 +928,10 @@ int htm_q4_matvec(const htm_q4_shape* s, const void* rec, const void* x, int32_t
         return htm_fail(HTM_E_INVALID, "%s: needs htm_q4_work_bytes of scratch", __func__);
     hipStream_t st = (hipStream_t)stream;
     float* y = p.splits > 1 ? (float*)work : out;
-    if (dtype == HTM_T_F32) mv_launch<float>(p, d, rec, x, xs, per, y, n, st);
-    else if (dtype == HTM_T_F16) mv_launch<__half>(p, d, rec, x, xs, per, y, n, st);
-    else mv_launch<__hip_bfloat16>(p, d, rec, x, xs, per, y, n, st);
+    const int r = dtype == HTM_T_F32   ? mv_launch<float>(p, d, rec, x, xs, per, y, n, st)
+                  : dtype == HTM_T_F16 ? mv_launch<__half>(p, d, rec, x, xs, per, y, n, st)
+                                       : mv_launch<__hip_bfloat16>(p, d, rec, x, xs, per, y, n, st);
+    if (r) return r;
     if (p.splits > 1)
         hipLaunchKernelGGL(q4_join_kernel, dim3((uint32_t)((n + 63) / 64)), dim3(256), 0, st, y, p.splits, n, out);
     return hipGetLastError() == hipSuccess ? HTM_OK : htm_fail(HTM_E_HIP, "q4 matvec launch failed");
