@@ -515,7 +515,7 @@ int htm_q4_matvec(const htm_q4_shape* shape, const void* d_records, const void* 
  * w * beam_stride + o; d_scores float [n_groups][beams_in]; d_live int32
  * [n_groups], clamped to 0..n_outputs, or NULL.  Out: float / int32 / int32
  * [n_groups][n_beams], best first.  1 <= beams_in, n_beams <= 64, beams_in *
- * n_outputs < 2^31.  d_work as for htm_q4_matvec. */
+ * n_outputs <= 2^30.  d_work as for htm_q4_matvec. */
 size_t htm_beam_work_bytes(int32_t n_groups, int32_t beams_in, int32_t n_beams, int32_t n_outputs);
 int htm_beam_select(const void* d_logits, int32_t dtype, int64_t group_stride, int64_t beam_stride,
                     const float* d_scores, const int32_t* d_live, int32_t n_groups, int32_t beams_in, int32_t n_beams,

@@ -8,7 +8,7 @@ kept beams' states go on from their parents'.  Kernels: csrc/beam.hip.
 """
 from __future__ import annotations
 
-import ctypes
+import array
 
 from . import _lib
 from ._lib import check
@@ -41,8 +41,8 @@ def beam_select(logits, scores, beams: int, live=None):
     groups, win, v = logits.shape
     dev = logits.device
     beams = int(beams)
-    if not 1 <= win <= MAX_BEAMS or not 1 <= beams <= MAX_BEAMS or v < 1 or win * v >= 2 ** 31 - 1:
-        raise ValueError("1..%d beams in and out, n_outputs >= 1 and beams_in * n_outputs < 2**31 (got %d, %d, %d)" %
+    if not 1 <= win <= MAX_BEAMS or not 1 <= beams <= MAX_BEAMS or v < 1 or win * v > 2 ** 30:
+        raise ValueError("1..%d beams in and out, n_outputs >= 1 and beams_in * n_outputs <= 2**30 (got %d, %d, %d)" %
                          (MAX_BEAMS, win, beams, v))
     if not isinstance(scores, torch.Tensor) or scores.dtype != torch.float32 or scores.device != dev or \
             scores.shape != (groups, win):
@@ -68,17 +68,6 @@ def beam_select(logits, scores, beams: int, live=None):
     return o_score, o_parent, o_bucket
 
 
-_ARRAYS = {}
-
-
-def _arrays(n):
-    """ctypes arrays for n buffers: sources, destinations, row bytes."""
-    if n not in _ARRAYS:
-        _ARRAYS[n] = (ctypes.c_void_p * n, ctypes.c_size_t * n)
-    p, s = _ARRAYS[n]
-    return p(), p(), s()
-
-
 def beam_reorder(buffers, parent, out=None):
     """Row (g, w) of every buffer becomes row (g, parent[g, w]).
 
@@ -102,7 +91,7 @@ def beam_reorder(buffers, parent, out=None):
     dev = parent.device
     parent = parent.contiguous()
     n = len(buffers)
-    src_p, dst_p, size = _arrays(n)
+    p = [0] * (3 * n)  # sources, destinations, row bytes
     for k, a in enumerate(buffers):
         b = dst[k]
         if not isinstance(a, torch.Tensor) or a.device != dev or not a.is_contiguous() or b is not a and (
@@ -113,7 +102,9 @@ def beam_reorder(buffers, parent, out=None):
         if not shape or shape[0] != rows and shape[:2] != (groups, beams):
             raise ValueError("a buffer must be [groups * beams, ...] or [groups, beams, ...] for %d groups of %d, got %s" %
                              (groups, beams, tuple(shape)))
-        src_p[k], dst_p[k], size[k] = a.data_ptr(), b.data_ptr(), a.nbytes // rows if rows else 0
+        p[k], p[n + k], p[2 * n + k] = a.data_ptr(), b.data_ptr(), a.nbytes // rows if rows else 0
+    p = array.array("Q", p)
+    at = p.buffer_info()[0]
     with _On(dev.index) as stream:
-        check(L.htm_beam_reorder(n, src_p, dst_p, size, parent.data_ptr(), groups, beams, stream))
+        check(L.htm_beam_reorder(n, at, at + 8 * n, at + 16 * n, parent.data_ptr(), groups, beams, stream))
     return dst

@@ -12,7 +12,8 @@
 #include "beam_dev.h"
 #include "htm_dev.h"
 
-#define BS_MAX 64  // beams
+#define BS_MAX 64              // beams
+#define BS_GROUPS (1 << 20)    // groups of one launch (of at most 1,024 threads each)
 
 __device__ __forceinline__ float up(float v) { return v; }
 __device__ __forceinline__ float up(__half v) { return __half2float(v); }
@@ -186,6 +187,7 @@ struct SelArgs {
     int64_t gs, bs;
     const float* score;
     const int32_t* live;
+    int64_t g0;  // the launch's first group
     int32_t win, wout, v;
     float* o_score;
     int32_t* o_parent;
@@ -224,7 +226,7 @@ __global__ void __launch_bounds__(1024) beam_small_kernel(SelArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint64_t small_sh[];  // tops, list: 64 a wave each
     __shared__ uint32_t count;
     const TopSh sh{small_sh, small_sh + blockDim.x, &count, (int)blockDim.x};
-    const int64_t g = blockIdx.x;
+    const int64_t g = a.g0 + blockIdx.x;
     const int lane = threadIdx.x & 63, w0 = (threadIdx.x >> 6) * R;
     const int n = live_of(a, g);
     const T* x = (const T*)a.x + g * a.gs + w0 * a.bs + lane;
@@ -294,7 +296,7 @@ __global__ void __launch_bounds__(1024) beam_select_kernel(SelArgs a, int parts,
     extern __shared__ __attribute__((aligned(16))) uint64_t select_sh[];  // tops, list, [win * v] logits, then scores
     const TopSh sh{select_sh, select_sh + blockDim.x, &count, BS_LIST};
     float* cand = reinterpret_cast<float*>(select_sh + blockDim.x + BS_LIST);
-    const int64_t g = blockIdx.x;
+    const int64_t g = a.g0 + blockIdx.x;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, nwave = blockDim.x >> 6;
     const int n = live_of(a, g), rows = nwave / parts, part = wave % parts, first = wave / parts;
     const T* x = (const T*)a.x + g * a.gs;
@@ -502,7 +504,7 @@ __global__ void __launch_bounds__(1024) beam_merge_kernel(SelArgs a, SelWork k) 
     __shared__ uint64_t tops[16 * 64], list[1024];
     __shared__ uint32_t count;
     const TopSh sh{tops, list, &count, 1024};
-    const int64_t g = blockIdx.x, n = (int64_t)a.win * k.chunks * a.wout;
+    const int64_t g = a.g0 + blockIdx.x, n = (int64_t)a.win * k.chunks * a.wout;
     const uint64_t* keys = k.keys + g * n;
     uint64_t best = 0;
 #pragma unroll 4
@@ -688,43 +690,45 @@ size_t htm_beam_work_bytes(int32_t groups, int32_t win, int32_t wout, int32_t v)
 }  // extern "C"
 
 template <typename T>
-static int select_launch(const SelArgs& a, int32_t groups, void* work, hipStream_t st) {
+static void select_launch(SelArgs a, int32_t groups, void* work, hipStream_t st) {
     const int64_t all = (int64_t)a.win * a.v;
-    if (sel_small(a.win, a.v)) {
-        const int each = (a.win + 15) / 16, waves = each > 2 ? (a.win + 3) / 4 : (a.win + each - 1) / each;
-        const auto small = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(groups), dim3(waves * 64), waves * 64 * 16, st, a);
-        };
-        if (each > 2) small(beam_small_kernel<T, 4, 4>);
-        else if (each == 2) a.v <= 256 ? small(beam_small_kernel<T, 2, 4>) : small(beam_small_kernel<T, 2, 8>);
-        else if (a.v <= 256) small(beam_small_kernel<T, 1, 4>);
-        else if (a.v <= 512) small(beam_small_kernel<T, 1, 8>);
-        else small(beam_small_kernel<T, 1, 16>);
-        return HTM_OK;
+    const bool small = sel_small(a.win, a.v);
+    SelWork k{};
+    if (!small && all > BS_ONE) {
+        k.chunks = sel_chunks(a.v);
+        const int64_t rows = (int64_t)groups * a.win;
+        k.sum = (double*)work;
+        k.keys = (uint64_t*)(k.sum + rows * k.chunks);
+        k.top = (float*)(k.keys + rows * k.chunks * a.wout);
+        for (int64_t r0 = 0; r0 < rows; r0 += 65535) {
+            const dim3 grid(k.chunks, (uint32_t)(rows - r0 < 65535 ? rows - r0 : 65535));
+            hipLaunchKernelGGL(beam_sums_kernel<T>, grid, dim3(256), 0, st, a, k, r0);
+            hipLaunchKernelGGL(beam_chunk_kernel<T>, grid, dim3(256), 0, st, a, k, r0);
+        }
     }
-    if (all <= BS_ONE) {
-        // (100 groups of 4 x 2,000: 256 threads 15.2 us, 512 12.7, 1,024 13.3; 2,000 groups: 39, 42, 90)
-        const int nt = groups < 512 ? 512 : 256;
-        int parts = 1;
-        while (parts * 2 * a.win <= nt / 64) parts *= 2;
-        const size_t lds = (size_t)(nt + BS_LIST) * sizeof(uint64_t) + (size_t)all * sizeof(float);
-        hipLaunchKernelGGL(beam_select_kernel<T>, dim3(groups), dim3(nt), lds, st, a, parts, 0xFFFFFFFFu / (uint32_t)a.v + 1u);
-        return HTM_OK;
+    for (int32_t g0 = 0; g0 < groups; g0 += BS_GROUPS) {
+        a.g0 = g0;
+        const dim3 grid(groups - g0 < BS_GROUPS ? groups - g0 : BS_GROUPS);
+        if (small) {
+            const int each = (a.win + 15) / 16, waves = each > 2 ? (a.win + 3) / 4 : (a.win + each - 1) / each;
+            const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(waves * 64), waves * 64 * 16, st, a); };
+            if (each > 2) go(beam_small_kernel<T, 4, 4>);
+            else if (each == 2) a.v <= 256 ? go(beam_small_kernel<T, 2, 4>) : go(beam_small_kernel<T, 2, 8>);
+            else if (a.v <= 256) go(beam_small_kernel<T, 1, 4>);
+            else if (a.v <= 512) go(beam_small_kernel<T, 1, 8>);
+            else go(beam_small_kernel<T, 1, 16>);
+        } else if (all <= BS_ONE) {
+            // (100 groups of 4 x 2,000: 256 threads 15.2 us, 512 12.7, 1,024 13.3; 2,000 groups: 39, 42, 90)
+            const int nt = groups < 512 ? 512 : 256;
+            int parts = 1;
+            while (parts * 2 * a.win <= nt / 64) parts *= 2;
+            const size_t lds = (size_t)(nt + BS_LIST) * sizeof(uint64_t) + (size_t)all * sizeof(float);
+            hipLaunchKernelGGL(beam_select_kernel<T>, grid, dim3(nt), lds, st, a, parts, 0xFFFFFFFFu / (uint32_t)a.v + 1u);
+        } else {
+            const int64_t keys = (int64_t)a.win * k.chunks * a.wout;
+            hipLaunchKernelGGL(beam_merge_kernel, grid, dim3(keys > 2048 ? 1024 : 256), 0, st, a, k);
+        }
     }
-    SelWork k;
-    k.chunks = sel_chunks(a.v);
-    const int64_t rows = (int64_t)groups * a.win;
-    k.sum = (double*)work;
-    k.keys = (uint64_t*)(k.sum + rows * k.chunks);
-    k.top = (float*)(k.keys + rows * k.chunks * a.wout);
-    for (int64_t r0 = 0; r0 < rows; r0 += 65535) {
-        const dim3 grid(k.chunks, (uint32_t)(rows - r0 < 65535 ? rows - r0 : 65535));
-        hipLaunchKernelGGL(beam_sums_kernel<T>, grid, dim3(256), 0, st, a, k, r0);
-        hipLaunchKernelGGL(beam_chunk_kernel<T>, grid, dim3(256), 0, st, a, k, r0);
-    }
-    const int64_t keys = (int64_t)a.win * k.chunks * a.wout;
-    hipLaunchKernelGGL(beam_merge_kernel, dim3(groups), dim3(keys > 2048 ? 1024 : 256), 0, st, a, k);
-    return HTM_OK;
 }
 
 extern "C" {
@@ -732,8 +736,8 @@ extern "C" {
 int htm_beam_select(const void* x, int32_t dtype, int64_t gs, int64_t bs, const float* score, const int32_t* live,
                     int32_t groups, int32_t win, int32_t wout, int32_t v, float* o_score, int32_t* o_parent,
                     int32_t* o_bucket, void* work, size_t work_bytes, void* stream) {
-    if (groups < 0 || win < 1 || win > BS_MAX || wout < 1 || wout > BS_MAX || v < 1 || (int64_t)win * v >= 0x7FFFFFFFll)
-        return htm_fail(HTM_E_INVALID, "%s: 1..64 beams in and out, outputs >= 1, beams_in * outputs < 2^31", __func__);
+    if (groups < 0 || win < 1 || win > BS_MAX || wout < 1 || wout > BS_MAX || v < 1 || (int64_t)win * v > (1ll << 30))
+        return htm_fail(HTM_E_INVALID, "%s: 1..64 beams in and out, outputs >= 1, beams_in * outputs <= 2^30", __func__);
     if (dtype != HTM_T_F32 && dtype != HTM_T_F16 && dtype != HTM_T_BF16)
         return htm_fail(HTM_E_INVALID, "%s: d_logits must be float32, float16 or bfloat16", __func__);
     if (!groups) return HTM_OK;
@@ -742,7 +746,7 @@ int htm_beam_select(const void* x, int32_t dtype, int64_t gs, int64_t bs, const 
     const size_t need = htm_beam_work_bytes(groups, win, wout, v);
     if (need && (!work || (uintptr_t)work % 8 || work_bytes < need))
         return htm_fail(HTM_E_INVALID, "%s: needs htm_beam_work_bytes of scratch, 8-byte aligned", __func__);
-    const SelArgs a{x, gs, bs, score, live, win, wout, v, o_score, o_parent, o_bucket};
+    const SelArgs a{x, gs, bs, score, live, 0, win, wout, v, o_score, o_parent, o_bucket};
     hipStream_t st = (hipStream_t)stream;
     if (dtype == HTM_T_F32) select_launch<float>(a, groups, work, st);
     else if (dtype == HTM_T_F16) select_launch<__half>(a, groups, work, st);

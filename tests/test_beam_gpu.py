@@ -58,6 +58,7 @@ SIZES = [  # groups, beams_in, beams, outputs
     (1, 1, 1, 1), (1, 1, 8, 480), (3, 8, 8, 480), (5, 4, 3, 7), (2, 1, 64, 5), (2, 64, 64, 3), (1, 64, 64, 1000),
     (7, 5, 5, 479), (33, 8, 8, 481), (2, 3, 17, 1001), (1, 16, 16, 8192), (2, 2, 8, 40000), (1, 1, 5, 100003),
     (3, 32, 32, 2047), (2, 7, 9, 4097), (300, 2, 4, 64), (1, 33, 31, 255), (1, 4, 4, 65536),
+    (2, 64, 64, 100), (1, 64, 64, 70000), (2, 3, 7, 1024), (1, 16, 33, 1000), (2, 32, 2, 512), (3, 17, 40, 512),
 ]
 
 
@@ -136,6 +137,10 @@ def test_strides_streams_and_many_groups(rt):
         assert all(torch.equal(p, q) for p, q in zip(a, b))
     x = torch.from_numpy(rng.standard_normal((70000, 1, 3))).float().cuda()  # more groups than one grid dimension holds
     check(rt, x, torch.zeros((70000, 1), device="cuda"), 2)
+    n = (1 << 20) + 5                                                        # and than one launch takes
+    x = torch.from_numpy(rng.standard_normal((n, 1, 2))).float().cuda()
+    got = rt.beam_select(x, torch.zeros((n, 1), device="cuda"), 1)
+    assert torch.equal(got[2][:, 0].long(), x[:, 0].argmax(1)) and torch.all(got[1] == 0)
 
 
 @pytest.mark.parametrize("v", [480, 30000])
