@@ -240,6 +240,11 @@ def model_forecast(fleet, beam_fleet, readout, cpu, horizon=LOOKAHEAD, bucket_va
         raise ValueError("the read-out must have one head and one matrix, or one for each of the %d streams" % g)
     if source not in ("tm_output", "col_confidence"):
         raise ValueError("source must be 'tm_output' or 'col_confidence'")
+    width = fleet.n_cells if source == "tm_output" else fleet.n_columns
+    if readout.n_inputs != width:
+        raise ValueError("the read-out has %d inputs, %s %d" % (readout.n_inputs, source, width))
+    if beam_fleet.device != fleet.device or readout.device != torch.device("cuda", fleet.device):
+        raise ValueError("the fleets and the read-out must be on one device")
     dev = f"cuda:{fleet.device}"
     c = fleet.config
     if bucket_values is None:

@@ -217,7 +217,7 @@ def test_forecast_refusals_and_no_bucket(rt, model, traces):
     f = rt.harness.model_forecast
     rec = np.array([10.0, 20.0])
     for bad in (dict(fleet=eng), dict(beam_fleet=fl), dict(beam_fleet=rt.HTMEngine.fleet(eng, 5)), dict(readout=cl.readout4()),
-                dict(horizon=0), dict(source="sp"), dict(bucket_values=np.zeros(3))):
+                dict(horizon=0), dict(source="sp"), dict(bucket_values=np.zeros(3)), dict(source="col_confidence")):
         with pytest.raises(ValueError):
             f(**{**dict(fleet=fl, beam_fleet=bf, readout=ro, cpu=rec), **bad})
     none = rt.Readout4(ro.records, ro.n_inputs, 1, ro.n_outputs, ro.group, live=torch.zeros(1, dtype=torch.int32, device="cuda"))
