@@ -459,8 +459,9 @@ int htm_cls_import_state(htm_classifier* cls, int32_t region, int32_t stream_beg
  * Records: uint8 [n_models][n_inputs][htm_q4_record_bytes], one input's weights:
  * per head the codes of its outputs (padded to a multiple of 32; the lower half
  * of a byte first), then per head ceil(padded / group) scales; padding is
- * ignored; scales are finite and at most 2^100.  Base address and d_x / d_pattern / d_out as the element type asks,
- * records 16-byte aligned. */
+ * ignored; scales are 0 or within 2^-110 .. 2^100.  Base address and d_x / d_pattern /
+ * d_out as the element type asks, records 16-byte aligned; d_out and d_work overlap
+ * nothing else of the call. */
 typedef struct {
     int32_t n_models;
     int32_t n_inputs;   /* 1..65536; patterns need a multiple of 32 */
@@ -476,8 +477,8 @@ typedef struct {
 size_t htm_q4_record_bytes(const htm_q4_shape* shape);
 /* Quantise d_weights (HTM_T_F32 / HTM_T_F64; element (m, i, h, o) at m * model_stride +
  * i * input_stride + h * head_stride + o) into d_records: scale = bfloat16(max|w| of
- * the group / 7), code = 8 + w / scale rounded to nearest even, within 1..15; a zero
- * stays exactly zero.  *d_bad (DEVICE int32, zeroed by the caller) is set to 1 if a
+ * the group / 7), 0 below 2^-110, code = 8 + w / scale rounded to nearest even, within
+ * 1..15; a zero stays exactly zero.  *d_bad (DEVICE int32, zeroed by the caller) is set to 1 if a
  * weight is infinite or NaN, or above 7 * 2^100 (its code is then meaningless). */
 int htm_q4_quantise(const htm_q4_shape* shape, const void* d_weights, int32_t dtype, int64_t model_stride,
                     int64_t input_stride, int64_t head_stride, void* d_records, int32_t* d_bad, void* stream);
@@ -496,7 +497,10 @@ int htm_q4_logits(const htm_q4_shape* shape, const void* d_records, const uint32
  * d_live: DEVICE int32 [n_models], clamped to 0..n_outputs; NULL: all. */
 int htm_q4_probabilities(const htm_q4_shape* shape, const void* d_records, const uint32_t* d_pattern,
                          int64_t pattern_stride, const int32_t* d_live, int32_t n_rows, float* d_out, void* stream);
-/* y for vectors of numbers (HTM_T_F32 / F16 / BF16, row r at r * x_stride elements).
+/* y for vectors of numbers (HTM_T_F32 / F16 / BF16, row r at r * x_stride elements).  An
+ * infinite number makes its row's outputs infinite, NaN where the weight is zero; other
+ * rows keep theirs.  With five and more rows a matrix what lies below 2^-126 in a
+ * number's 8-bit parts, a product or a sum may count as zero.
  * d_work: DEVICE scratch of htm_q4_work_bytes (may be NULL when that is 0), not
  * shared with a call that may run at the same time. */
 size_t htm_q4_work_bytes(const htm_q4_shape* shape, int32_t n_rows);
@@ -514,7 +518,7 @@ int htm_q4_matvec(const htm_q4_shape* shape, const void* d_records, const void* 
  * d_logits (HTM_T_F32 / F16 / BF16): element (g, w, o) at g * group_stride +
  * w * beam_stride + o; d_scores float [n_groups][beams_in]; d_live int32
  * [n_groups], clamped to 0..n_outputs, or NULL.  Out: float / int32 / int32
- * [n_groups][n_beams], best first.  1 <= beams_in, n_beams <= 64, beams_in *
+ * [n_groups][n_beams], best first, apart from what is read.  1 <= beams_in, n_beams <= 64, beams_in *
  * n_outputs <= 2^30.  d_work as for htm_q4_matvec. */
 size_t htm_beam_work_bytes(int32_t n_groups, int32_t beams_in, int32_t n_beams, int32_t n_outputs);
 int htm_beam_select(const void* d_logits, int32_t dtype, int64_t group_stride, int64_t beam_stride,

@@ -38,6 +38,8 @@ def beam_select(logits, scores, beams: int, live=None):
     code = dtype_code(logits.dtype) if isinstance(logits, torch.Tensor) else -1
     if code not in (0, 2, 3) or logits.dim() != 3 or not logits.is_cuda:
         raise ValueError("logits must be a float32, float16 or bfloat16 CUDA tensor [groups, beams_in, n_outputs]")
+    if torch.is_grad_enabled() and logits.requires_grad:
+        raise ValueError("a selection has no gradient: detach the logits")
     groups, win, v = logits.shape
     dev = logits.device
     beams = int(beams)

@@ -21,6 +21,7 @@
 
 #define Q4_NT 256
 #define Q4_MAX_SCALE 1.2676506002282294e30  // 2^100: a scale times 2^24 stays finite (Q4Acc)
+#define Q4_MIN_SCALE 7.7037197775489434e-34 // 2^-110: its lower four bits are a normal number (q4_mfma_kernel)
 
 int q4_dims(const htm_q4_shape* s, const char* who, Q4Dims* d) {
     if (!s) return htm_fail(HTM_E_INVALID, "%s: null shape", who);
@@ -77,7 +78,7 @@ __global__ void __launch_bounds__(Q4_NT) q4_quantise_kernel(Q4Dims d, const T* _
         }
         odd |= amax > 7.0 * Q4_MAX_SCALE;
         const float s0 = (float)(amax / 7.0);
-        const uint32_t sb = s0 >= 1.17549435e-38f && !odd ? bf16_round(s0) : 0u;
+        const uint32_t sb = (double)s0 >= Q4_MIN_SCALE && !odd ? bf16_round(s0) : 0u;
         const double s = (double)bf16_up(sb);
         uint8_t* r = rec + row * (int64_t)d.pitch;
         for (int o = o0; o < o1; o += 2) {
@@ -519,7 +520,9 @@ __global__ void __launch_bounds__(MV_NT, NX == 4 ? 3 : 4)
 // number takes one (bfloat16), two (float16) or three (float32) bfloat16 parts,
 // so that every product in the sum is exact and only float32 sums round, as in the
 // kernel above, while a weight costs some 4.4 instructions for all 16 rows
-// instead of 3 and one for each row.
+// instead of 3 and one for each row.  Matrix instructions take what lies below
+// float32's normal numbers as zero: scales are kept off that range, and of x and the
+// products 2^-126 may be lost.
 //
 // One workgroup per (16 rows of one matrix, 16 half blocks, range of inputs).  The
 // tile's inputs are listed as above, with their numbers' parts in LDS; its waves
@@ -574,18 +577,24 @@ __global__ void __launch_bounds__(MM_NT, 2)
     };
     fetch(k0);
     for (int t0 = k0; t0 < k1; t0 += MM_TILE) {
-        bool some = false;
+        bool some = false, odd = false;
 #pragma unroll
-        for (int r = 0; r < MM_ROWS; r++) some |= mine[r] != 0.0f;
-        const uint64_t bal = __ballot(some);
-        if (lane == 0) wsum[wave] = (uint32_t)__popcll(bal);
+        for (int r = 0; r < MM_ROWS; r++) {
+            some |= mine[r] != 0.0f;
+            odd |= !(fabsf(mine[r]) < INFINITY);
+        }
+        const uint64_t bal = __ballot(some), odds = __ballot(odd);
+        if (lane == 0) wsum[wave] = (uint32_t)__popcll(bal) | (odds ? 0x10000u : 0u);
         __syncthreads();
         uint32_t at = (uint32_t)__popcll(bal & ((1ull << lane) - 1ull)), m = 0;
 #pragma unroll
         for (int k = 0; k < MM_NT / 64; k++) {
-            if (k < wave) at += wsum[k];
-            m += wsum[k];
+            const uint32_t c = wsum[k];
+            if (k < wave) at += c & 0xFFFFu;
+            m += c;
         }
+        const bool wild = m > 0xFFFFu;  // an infinity or a NaN among the tile's numbers
+        m &= 0xFFFFu;
         // up to a multiple of 32 behind the list: the tile's first input, times zero
         const uint32_t pad = (32u - (m & 31u)) & 31u;
         const bool fill = threadIdx.x < pad;
@@ -621,6 +630,16 @@ __global__ void __launch_bounds__(MM_NT, 2)
             for (int p = 0; p < P; p++)
                 a[p] = *reinterpret_cast<const bf16x8*>(xa + (p * MM_ROWS + (lane & 15)) * MM_PITCH + q8);
             __builtin_amdgcn_sched_barrier(0);  // (every load is under way before the first is waited for)
+            // (the scale's lower part may be zero where the weight is not: infinity meets the upper one alone)
+            u32x4 fin = __builtin_bit_cast(u32x4, a[0]);
+            if (wild) {
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    if ((fin[k] & 0x7F80u) == 0x7F80u) fin[k] &= 0xFFFF0000u;
+                    if ((fin[k] & 0x7F800000u) == 0x7F800000u) fin[k] &= 0x0000FFFFu;
+                }
+            }
+            const bf16x8 a0 = __builtin_bit_cast(bf16x8, fin);
             float hi[8], lo[8];
 #pragma unroll
             for (int r = 0; r < 8; r++) {
@@ -643,17 +662,18 @@ __global__ void __launch_bounds__(MM_NT, 2)
                     for (int p = 0; p < 4; p++) {
                         const uint32_t u = n < 2 ? w[p] : w[p] >> 8;
                         const half2_t q2 = as_half2(n & 1 ? and_or(u, 0x00F000F0u, e72) : and_or(u, 0x000F000Fu, e1032)) - bias;
-                        const float a0 = __builtin_fmaf((float)q2.x, hi[2 * p], 0.0f);
-                        const float a1 = __builtin_fmaf((float)q2.y, hi[2 * p + 1], 0.0f);
-                        const float b0 = __builtin_fmaf((float)q2.x, lo[2 * p], 0.0f);
-                        const float b1 = __builtin_fmaf((float)q2.y, lo[2 * p + 1], 0.0f);
-                        bh[p] = __builtin_amdgcn_perm(__float_as_uint(a1), __float_as_uint(a0), 0x07060302u);
-                        bl[p] = __builtin_amdgcn_perm(__float_as_uint(b1), __float_as_uint(b0), 0x07060302u);
+                        const float h0 = __builtin_fmaf((float)q2.x, hi[2 * p], 0.0f);
+                        const float h1 = __builtin_fmaf((float)q2.y, hi[2 * p + 1], 0.0f);
+                        const float l0 = __builtin_fmaf((float)q2.x, lo[2 * p], 0.0f);
+                        const float l1 = __builtin_fmaf((float)q2.y, lo[2 * p + 1], 0.0f);
+                        bh[p] = __builtin_amdgcn_perm(__float_as_uint(h1), __float_as_uint(h0), 0x07060302u);
+                        bl[p] = __builtin_amdgcn_perm(__float_as_uint(l1), __float_as_uint(l0), 0x07060302u);
                     }
                     const int j = g * 4 + n;
 #pragma unroll
                     for (int p = 0; p < P; p++) {
-                        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[p], __builtin_bit_cast(bf16x8, bl), acc[j], 0, 0, 0);
+                        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p ? a[p] : a0, __builtin_bit_cast(bf16x8, bl), acc[j], 0, 0,
+                                                                         0);
                         acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[p], __builtin_bit_cast(bf16x8, bh), acc[j], 0, 0, 0);
                     }
                 }

@@ -214,10 +214,14 @@ class Readout4:
 
     def matvec(self, x, out=None):
         """y of vectors of numbers [rows, n_inputs], float32 / float16 /
-        bfloat16 (the engine's "col_confidence", an averaged activity)."""
+        bfloat16 (the engine's "col_confidence", an averaged activity).  An
+        infinite number makes its row's outputs infinite (NaN where the weight
+        is zero), a NaN makes them NaN; other rows keep theirs."""
         import torch
         if not isinstance(x, torch.Tensor) or dtype_code(x.dtype) not in (0, 2, 3):
             raise ValueError("x must be a float32, float16 or bfloat16 tensor [rows, n_inputs]")
+        if x.requires_grad and torch.is_grad_enabled():
+            raise ValueError("a frozen read-out has no gradient: detach x")
         v, n, stride = self._rows(x, self.n_inputs, "x")
         y = self._out(out, n)
         nb = self._L.htm_q4_work_bytes(self._pshape, n)

@@ -111,6 +111,61 @@ def test_masked_infinite_and_nan(rt, v):
     check(rt, x, s, 8, live)
 
 
+@pytest.mark.parametrize("win,v", [(1, 200), (64, 256), (8, 480), (16, 1000), (3, 2500), (5, 60000)])
+def test_more_candidates_than_a_short_list(rt, win, v):
+    """Every 64th output low, in order or against it: nearly all candidates lie above what 64 of them are sure to reach."""
+    rng = np.random.default_rng(v)
+    x = rng.standard_normal((4, win, v))
+    x[1] = np.sort(x[1], -1)
+    x[2] = np.sort(x[2], -1)[:, ::-1]
+    x[3] = np.round(x[3])
+    x[..., 5::64] -= 60
+    x = torch.from_numpy(x.copy()).float().cuda()
+    s = torch.from_numpy(-rng.random((4, win))).float().cuda()
+    for beams in (64, 33, 2):
+        check(rt, x, s, beams)
+
+
+def test_calls_at_once(rt):
+    """Selections and in-place moves on two streams at the same time."""
+    rng = np.random.default_rng(5)
+    work = []
+    for k in range(2):
+        x = torch.from_numpy(rng.standard_normal((64, 4, 30000))).float().cuda()
+        s = torch.from_numpy(-rng.random((64, 4))).float().cuda()
+        state = torch.from_numpy(rng.integers(0, 1 << 30, (256, 5000))).cuda()
+        want = rt.beam_select(x, s, 4)
+        work.append((x, s, state, want, rt.beam_reorder([state], want[1], out=[torch.empty_like(state)])[0]))
+    torch.cuda.synchronize()
+    got = []
+    for x, s, state, _, _ in work:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            r = rt.beam_select(x, s, 4)
+            got.append((r, rt.beam_reorder([state.clone()], r[1])[0]))
+    torch.cuda.synchronize()
+    for (r, moved), (_, _, _, want, at) in zip(got, work):
+        assert all(torch.equal(p, q) for p, q in zip(r, want)) and torch.equal(moved, at)
+
+
+def test_reorder_in_place_captured_into_a_graph(rt):
+    rng = np.random.default_rng(6)
+    first = torch.from_numpy(rng.integers(0, 99, (24, 1037), dtype=np.uint8)).cuda()
+    a, b = first.clone(), first.clone()
+    p = torch.from_numpy(rng.integers(0, 8, (3, 8)).astype(np.int32)).cuda()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        rt.beam_reorder([b.clone()], p)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        rt.beam_reorder([a], p)
+    for _ in range(5):
+        p.copy_(torch.from_numpy(rng.integers(0, 8, (3, 8)).astype(np.int32)))
+        g.replay()
+        rt.beam_reorder([b], p)
+        torch.cuda.synchronize()
+        assert torch.equal(a, b)
+
+
 def test_scores_of_very_different_size(rt):
     x = torch.zeros((1, 3, 8), device="cuda")
     x[0, 0, 5], x[0, 1, 2] = 80.0, -300.0
@@ -180,6 +235,8 @@ def test_select_refusals(rt):
                  (torch.zeros((1, 65, 2), device="cuda"), torch.zeros((1, 65), device="cuda"), 2)):
         with pytest.raises(ValueError):
             rt.beam_select(*args)
+    with pytest.raises(ValueError, match="gradient"):
+        rt.beam_select(x.clone().requires_grad_(), s, 2)
     for live in (torch.ones(2, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda"), torch.ones(2, dtype=torch.int32)):
         with pytest.raises(ValueError):
             rt.beam_select(x, s, 2, live=live)

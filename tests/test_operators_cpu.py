@@ -87,6 +87,26 @@ def test_beam_arguments_refused(rt):
     assert L.htm_copy_streams(None, None, p, None) == INV
 
 
+def test_scratch_refused(rt):
+    """Too little scratch, none, or at an odd address, wherever a call needs some."""
+    L = rt._lib.lib()
+    INV = rt._lib.HTM_E_INVALID
+    p = ctypes.c_void_p(4096)
+    for rows, dtype in ((1, 0), (2, 2), (4, 3), (16, 0)):
+        s = shape(rt, inputs=24576, heads=1, outputs=480)
+        need = L.htm_q4_work_bytes(ref(s), rows)
+        assert need and need % (4 * rows * 480) == 0
+        for work, nb in ((None, need), (p, need - 1), (p, 0), (ctypes.c_void_p(4098), need)):
+            assert L.htm_q4_matvec(ref(s), p, p, dtype, 24576, rows, p, work, nb, None) == INV
+    assert L.htm_q4_work_bytes(ref(shape(rt)), 0) == 0 and L.htm_q4_work_bytes(None, 1) == 0
+    for win, wout, v in ((1, 1, 8193), (64, 64, 1000), (8, 8, 1 << 20)):
+        need = L.htm_beam_work_bytes(3, win, wout, v)
+        assert need >= 3 * win * wout * 8
+        for work, nb in ((None, need), (p, need - 1), (p, 0), (ctypes.c_void_p(4100), need)):
+            assert L.htm_beam_select(p, 0, win * v, v, p, None, 3, win, wout, v, p, p, p, work, nb, None) == INV
+    assert L.htm_beam_work_bytes(3, 8, 8, 480) == 0 and L.htm_beam_work_bytes(0, 8, 8, 1 << 20) == 0
+
+
 def test_tensors_off_the_gpu_refused(rt):
     with pytest.raises(ValueError):
         rt.Readout4(torch.zeros((1, 32, 64), dtype=torch.uint8), 32, 1, 40)

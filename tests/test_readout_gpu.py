@@ -3,7 +3,13 @@ against float64 sums of the same weights.
 
 Tolerance: a weight s * (c - 8) is exact in float32 (8 + 4 bits); a product
 with x rounds once and a sum of n terms n times at most, in whatever order, so
-|y - y64| <= (n + 2) * 2^-24 * sum |x w| per output.  softmax: an error d of
+|y - y64| <= (n + 2) * 2^-24 * sum |x w| per output.  matvec of five and more rows
+a matrix adds up to six exact products a weight instead (their absolute values
+sum to at most 1 + 2^-6 times |x w|) and meets the same bound by the matrix
+instructions' order, which rounds once per 8 or more products.  logits and
+probabilities sum s * c and take 8 * sum s off at the end: what can be proved
+has sum s (c + 8) in place of sum |x w|; they are held to the smaller bound here,
+since n roundings do not all fall to one side.  softmax: an error d of
 the logits moves a probability by a factor within exp(+-2 d), expf and the
 division round to 3 * 2^-23 and the sum of k terms to k * 2^-24."""
 import numpy as np
@@ -21,14 +27,14 @@ def up(n, to):
     return -(-n // to) * to
 
 
-def make(rt, models, inputs, heads, outputs, group, seed=0):
+def make(rt, models, inputs, heads, outputs, group, seed=0, size=1.0):
     """A read-out of random codes and scales, and its float64 weights [models, inputs, heads, outputs]."""
     rng = np.random.default_rng(seed)
     padded = up(outputs, 32)
     groups = -(-padded // group)
     per = rt.Readout4.record_bytes(models, inputs, heads, outputs, group)
     rec = rng.integers(0, 256, (models, inputs, per), dtype=np.uint8)
-    s32 = (rng.random((models, inputs, heads, groups)) * 0.1 + 0.001).astype(np.float32)
+    s32 = ((rng.random((models, inputs, heads, groups)) * 0.1 + 0.001) * size).astype(np.float32)
     bits = (s32.view(np.uint32) >> 16).astype(np.uint16)
     nb = heads * padded // 2
     rec[:, :, nb:nb + 2 * heads * groups] = bits.reshape(models, inputs, -1).view(np.uint8)
@@ -174,6 +180,93 @@ def test_infinite_and_nan_inputs_stay_in_their_row(rt):
     assert torch.all(got[1].isnan()) and not torch.any(got[3].isfinite() & torch.from_numpy(w[0, 200, :, :] != 0).cuda())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 2, 4, 5, 20])
+def test_an_infinite_input_by_the_formula(rt, rows, dtype):
+    """inf * w is an infinity of w's sign, NaN where w is zero, whatever the bits of the scales."""
+    r, w = make(rt, 1, 300, 2, 77, 64)
+    x = torch.from_numpy(np.random.default_rng(10).standard_normal((rows, 300))).to(dtype).cuda()
+    x[rows - 1, 290], x[0, 7] = float("-inf"), float("inf")
+    got = r.matvec(x).cpu().numpy()
+    with np.errstate(invalid="ignore"):
+        for row, k in ((rows - 1, 290), (0, 7)) if rows > 1 else ():
+            assert np.array_equal(got[row], float(x[row, k]) * w[0, k], equal_nan=True)
+        if rows == 1:
+            assert np.array_equal(got[0], np.inf * w[0, 7] - np.inf * w[0, 290], equal_nan=True)
+
+
+@pytest.mark.parametrize("size", [2.0 ** -122, 2.0 ** -100, 2.0 ** 100])
+@pytest.mark.parametrize("rows", [1, 3, 6, 17])
+def test_small_and_large_numbers(rt, rows, size):
+    """The same bound far from 1; below float32's normal numbers 2^-149 more a product (each of the six exact ones).
+    Five and more rows go through matrix instructions, which take an operand or a result below 2^-126 as zero: of a
+    number's three parts that loses less than 3 * 2^-126 times the weight, of the six products and of the six sums
+    less than 2^-126 each."""
+    r, w = make(rt, 1, 700, 1, 96, 32)
+    x = torch.from_numpy(np.random.default_rng(11).standard_normal((rows, 700)) * size).float()
+    y, tol = expect(w, x.double().numpy())
+    lost = (12 + 3 * np.abs(w).max()) * 700 * 2.0 ** -126 if rows >= 5 else 6 * 700 * 2.0 ** -149
+    near(r.matvec(x.cuda()), y, tol + lost)
+
+
+@pytest.mark.parametrize("size", [2.0 ** -100, 2.0 ** 103])
+@pytest.mark.parametrize("rows", [1, 3, 6])
+def test_small_and_large_scales(rt, rows, size):
+    """Scales next to both ends of their range, 2^-110 .. 2^100."""
+    r, w = make(rt, 1, 700, 1, 96, 32, size=size)
+    x = torch.from_numpy(np.random.default_rng(15).standard_normal((rows, 700)) / size).float()
+    near(r.matvec(x.cuda()), *expect(w, x.double().numpy()))
+    p = np.random.default_rng(16).random((rows, 704)) < 0.1
+    r, w = make(rt, 1, 704, 1, 96, 32, size=size)
+    near(r.logits(words(p)), *expect(w, p.astype(np.float64)))
+
+
+@pytest.mark.parametrize("rows,models", [(36, 2), (66000, 66000), (66000, 1), (140000, 7)])
+def test_matvec_of_many_rows(rt, rows, models):
+    """Passes behind the first, and more rows than one grid dimension holds, for both kernels."""
+    r, w = make(rt, models, 64, 1, 40, 32)
+    x = torch.from_numpy(np.random.default_rng(12).standard_normal((rows, 64))).float()
+    got = r.matvec(x.cuda()).cpu().numpy().astype(np.float64)
+    f = x.double().numpy().reshape(models, rows // models, 64)
+    y = (f @ w[:, :, 0]).reshape(rows, 1, 40)
+    tol = (np.abs(f) @ np.abs(w[:, :, 0])).reshape(rows, 1, 40) * (64 + 2) * EPS
+    assert np.all(np.abs(got - y) <= tol)
+
+
+@pytest.mark.parametrize("rows,models", [(66000, 66000), (66000, 1)])
+def test_logits_of_many_rows(rt, rows, models):
+    r, w = make(rt, models, 64, 1, 40, 32)
+    x = np.random.default_rng(13).random((rows, 64)) < 0.2
+    got = r.logits(words(x)).cpu().numpy().astype(np.float64)
+    f = x.astype(np.float64).reshape(models, rows // models, 64)
+    y = (f @ w[:, :, 0]).reshape(rows, 1, 40)
+    tol = (f @ np.abs(w[:, :, 0])).reshape(rows, 1, 40) * (64 + 2) * EPS
+    assert np.all(np.abs(got - y) <= tol)
+    p = r.probabilities(words(x)).cpu().numpy()
+    assert np.all(np.abs(p.sum(-1) - 1) <= 1e-5) and np.array_equal(p.argmax(-1), got.argmax(-1))
+
+
+def test_records_past_32_bits(rt):
+    """The last models of 5.2 GB of records: offsets of more than 32 bits."""
+    ni, no, nm = 16384, 480, 1170
+    per = rt.Readout4.record_bytes(nm, ni, 1, no)
+    rec = torch.zeros((nm, ni, per), dtype=torch.uint8, device="cuda")
+    assert rec.numel() > 2 ** 32
+    one, w = make(rt, 2, ni, 1, no, 32)
+    assert one.records.shape[2] == per
+    rec[-2:] = one.records
+    r = rt.Readout4(rec, ni, 1, no)
+    rng = np.random.default_rng(14)
+    x = rng.random((nm, ni)) < 0.01
+    got = r.logits(words(x))
+    assert torch.all(got[:-2] == 0)
+    assert torch.equal(got[-2:], one.logits(words(x[-2:])))
+    near(got[-2:], *expect(w, x[-2:].astype(np.float64)))
+    for rows in (1, 5):
+        v = torch.from_numpy(rng.standard_normal((nm * rows, ni)).astype(np.float32) * (rng.random(ni) < 0.05)).float()
+        near(r.matvec(v.cuda())[-2 * rows:], *expect(w, v[-2 * rows:].double().numpy()))
+
+
 def test_deterministic_and_on_another_stream(rt):
     r, _ = make(rt, 1, 24576, 7, 480, 32)
     rng = np.random.default_rng(7)
@@ -265,6 +358,25 @@ def test_quantize_refuses_nonfinite(rt):
             rt.Readout4.quantize(w)
 
 
+def test_quantize_below_its_range(rt):
+    """A group whose scale would lie below 2^-110 is zero; the next one at 2^-110 is not."""
+    w = torch.zeros((1, 4, 1, 64), device="cuda", dtype=torch.float64)
+    w[0, 1, 0, :32], w[0, 1, 0, 32:] = 6.99 * 2.0 ** -110, 7 * 2.0 ** -110
+    y = rt.Readout4.quantize(w).matvec(torch.full((1, 4), 2.0 ** 60, device="cuda"))[0, 0]
+    assert torch.all(y[:32] == 0) and torch.all(y[32:] == 7 * 2.0 ** -50)
+
+
+def test_quantize_refuses_above_its_range(rt):
+    for dtype in (torch.float32, torch.float64):
+        w = torch.zeros((1, 4, 1, 40), device="cuda", dtype=dtype)
+        w[0, 2, 0, 39] = -7 * 2.0 ** 100
+        r = rt.Readout4.quantize(w)
+        assert float(r.matvec(torch.ones((1, 4), device="cuda"))[0, 0, 39]) == -7 * 2.0 ** 100
+        w[0, 2, 0, 39] = 7.01 * 2.0 ** 100
+        with pytest.raises(ValueError, match="2\\*\\*100"):
+            rt.Readout4.quantize(w)
+
+
 def test_from_a_trained_classifier(rt, traces):
     """The read-out of a trained classifier answers as its own weights do, and finds the classifier's best bucket."""
     steps = [1, 2, 3]
@@ -318,6 +430,10 @@ def test_refusals(rt):
                 torch.zeros((3, 96), device="cuda"), torch.zeros((2, 96))):
         with pytest.raises(ValueError):
             r.matvec(bad)
+    with pytest.raises(ValueError, match="gradient"):
+        r.matvec(torch.zeros((2, 96), device="cuda", requires_grad=True))
+    with torch.no_grad():
+        r.matvec(torch.zeros((2, 96), device="cuda", requires_grad=True))
     for bad in (torch.ones(1, dtype=torch.int32, device="cuda"), torch.ones(2, device="cuda"), torch.ones(2, dtype=torch.int32)):
         with pytest.raises(ValueError):
             r.probabilities(p, bad)
