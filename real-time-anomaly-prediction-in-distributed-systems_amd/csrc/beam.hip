@@ -220,7 +220,9 @@ __device__ __forceinline__ void put_rest(const SelArgs& a, int64_t g, int taken)
 // and no barrier before it.  What it costs is the chain of one wave: load, the
 // largest, E exponentials, the sum, a logarithm, the scores.  Measured, us, 8 x
 // 480 -> 8: one group 5.6 (the logits in LDS, between barriers: 10.4), 512 groups
-// 8.2 (13.6), 4,096 groups 35 (54); two beams a wave 7.0, 9.0, 33.
+// 8.2 (13.6), 4,096 groups 30 to 34 (54); two beams a wave 7.0, 9.0, 33.  Many groups
+// are bound by float64 instructions: 2.0e7 of a wave, 600 for each beam, are 32 us
+// of issue; the 63 MB take 13.
 template <typename T, int R, int E>
 __global__ void __launch_bounds__(1024) beam_small_kernel(SelArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint64_t small_sh[];  // tops, list: 64 a wave each
@@ -283,7 +285,8 @@ __global__ void __launch_bounds__(1024) beam_small_kernel(SelArgs a) {
 }
 
 // More (beams_in * n_outputs <= BS_ONE): one workgroup per group, the logits read
-// once into LDS.  parts waves share a beam.
+// once into LDS.  parts waves share a beam.  100 groups of 4 x 2,000: 12.7 us, the chain of
+// the same steps with a barrier behind each.
 #define BS_ONE 8192
 #define BS_LIST 512
 template <typename T>
@@ -400,7 +403,10 @@ __global__ void __launch_bounds__(1024) beam_select_kernel(SelArgs a, int parts,
     put_rest(a, g, taken);
 }
 
-// Many candidates: chunks of BS_CHUNK of a beam's outputs, three launches.
+// Many candidates: chunks of BS_CHUNK of a beam's outputs, three launches, since a
+// beam's sum is needed before its first score.  4 groups of 16 x 32,768 bfloat16 -> 16:
+// 5.8, 11 and 6 us in 21 us, each the latency of a few loads, sums and a selection;
+// the 4 MB of logits are read again from the caches.
 #define BS_CHUNK 4096
 struct SelWork {
     float* top;      // [groups * win * chunks] the chunks' largest logits, +infinity where there is a NaN
@@ -519,7 +525,10 @@ __global__ void __launch_bounds__(1024) beam_merge_kernel(SelArgs a, SelWork k) 
 // All buffers of a call in one launch: block b belongs to buffer k with first[k]
 // <= b < first[k + 1].  A buffer's rows are moved in its widest unit (16 bytes
 // down to 1, what its size and addresses divide by); 2^lanes[k] threads share a
-// row, four units each, all read before the first is written.
+// row, four units each, all read before the first is written.  Bound by memory:
+// 32,768 rows of 9,856 B, 8 beams a group, parents at random: 109 us for 535 MB read
+// and written, 4.9 TB/s, as fast as a plain copy; 323 MB of a fleet's states, some 30 KB
+// a row over several buffers, 62 us.
 struct MoveArgs {
     RowMoves m;
     uint32_t first[HTM_BEAM_BUFFERS + 1];
@@ -588,7 +597,10 @@ __global__ void __launch_bounds__(256) rows_copy_kernel(MoveArgs a) {
 
 // In place: a thread owns a unit's place in all W rows of a group, reads the
 // parents' and only then writes, so that no other thread's data is involved and
-// nothing is kept beside the buffers.  Rows that stay are not touched.
+// nothing is kept beside the buffers.  Rows that stay are not touched.  The same rows
+// as above, only those that move written: 2 beams 115 us, 8 92 us (5.4 TB/s), 16 103
+// us, 32 139 us, 64 187 us (2.8 TB/s): the more rows a thread holds, the fewer waves
+// a CU does.
 template <typename U, int W>
 __device__ __forceinline__ void move_in(const MoveArgs& a, int k, uint32_t block) {
     const int log = a.lanes[k], t = threadIdx.x & ((1 << log) - 1);

@@ -57,49 +57,64 @@ __device__ __forceinline__ float x_up(__half v) { return __half2float(v); }
 __device__ __forceinline__ float x_up(__hip_bfloat16 v) { return __bfloat162float(v); }
 
 // ---------------------------------------------------------------- quantiser
-// One thread per group of one (model, input, head): two passes over its
-// weights, the largest magnitude and then the codes.
+// One workgroup per record, 16 lanes per group: a lane holds neighbouring pairs of
+// its weights, a byte of codes each, so that weights and codes go by whole lines.
+// 2 x 24,576 x 7 x 480: float64 483 us (2.9 TB/s), float32 452 us, which the
+// divisions bound (a group a thread, whose reads and writes share no line: 5.1 and
+// 6.0 ms).
 template <typename T>
 __global__ void __launch_bounds__(Q4_NT) q4_quantise_kernel(Q4Dims d, const T* __restrict__ w, int64_t ms, int64_t is,
                                                             int64_t hs, uint8_t* __restrict__ rec, int32_t* bad) {
-    const int64_t per = (int64_t)d.nh * d.ngrp;
-    const int64_t total = (int64_t)d.nm * d.ni * per;
-    for (int64_t t = (int64_t)blockIdx.x * Q4_NT + threadIdx.x; t < total; t += (int64_t)gridDim.x * Q4_NT) {
-        const int64_t row = t / per;
-        const int k = (int)(t - row * per), h = k / d.ngrp, g = k - h * d.ngrp;
-        const T* src = w + (row / d.ni) * ms + (row % d.ni) * is + (int64_t)h * hs;
-        const int o0 = g * d.group, o1 = min(o0 + d.group, d.nblk * Q4_BLK);
-        double amax = 0.0;
-        bool odd = false;
-        for (int o = o0; o < min(o1, d.no); o++) {
-            const double a = fabs((double)src[o]);
-            odd |= !(a <= 1.7976931348623157e308);
-            amax = fmax(amax, a);
-        }
-        odd |= amax > 7.0 * Q4_MAX_SCALE;
-        const float s0 = (float)(amax / 7.0);
-        const uint32_t sb = (double)s0 >= Q4_MIN_SCALE && !odd ? bf16_round(s0) : 0u;
-        const double s = (double)bf16_up(sb);
+    const int64_t rows = (int64_t)d.nm * d.ni;
+    const int per = d.nh * d.ngrp, lane = threadIdx.x & 15, padded = d.nblk * Q4_BLK;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const int64_t model = row / d.ni;
+        const T* in = w + model * ms + (row - model * d.ni) * is;
         uint8_t* r = rec + row * (int64_t)d.pitch;
-        for (int o = o0; o < o1; o += 2) {
-            uint32_t c[2] = {8u, 8u};
-            for (int j = 0; j < 2; j++)
-                if (o + j < d.no && s > 0.0) {
-                    const double q = fmin(fmax(rint((double)src[o + j] / s), -7.0), 7.0);
-                    c[j] = (uint32_t)(8 + (int)q);
+        for (int k = threadIdx.x >> 4; k < per; k += Q4_NT / 16) {
+            const int h = k / d.ngrp, g = k - h * d.ngrp, o0 = g * d.group + 2 * lane;
+            const T* src = in + (int64_t)h * hs;
+            T v[4][2];
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) v[q][j] = q * 32 < d.group && o0 + q * 32 + j < d.no ? src[o0 + q * 32 + j] : (T)0;
+            double amax = 0.0;
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const double a = fabs((double)v[q][j]);
+                    amax = a <= 7.0 * Q4_MAX_SCALE ? fmax(amax, a) : INFINITY;  // (NaN among them)
                 }
-            r[((size_t)h * d.nblk * Q4_BLK + o) >> 1] = (uint8_t)(c[0] | (c[1] << 4));
+#pragma unroll
+            for (int m = 8; m; m >>= 1) amax = fmax(amax, __shfl_xor(amax, m));
+            const bool odd = amax == INFINITY;
+            const float s0 = (float)(amax / 7.0);
+            const uint32_t sb = (double)s0 >= Q4_MIN_SCALE && !odd ? bf16_round(s0) : 0u;
+            const double s = (double)bf16_up(sb);
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const int o = o0 + q * 32;
+                if (q * 32 >= d.group || o >= padded) break;
+                uint32_t c[2];
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+                    c[j] = sb ? (uint32_t)(8 + (int)fmin(fmax(rint((double)v[q][j] / s), -7.0), 7.0)) : 8u;
+                r[((uint32_t)(h * padded) + o) >> 1] = (uint8_t)(c[0] | (c[1] << 4));
+            }
+            if (lane == 0) {
+                reinterpret_cast<uint16_t*>(r + d.scales)[k] = (uint16_t)sb;
+                if (odd) *bad = 1;
+            }
         }
-        reinterpret_cast<uint16_t*>(r + d.scales)[h * d.ngrp + g] = (uint16_t)sb;
-        if (odd) *bad = 1;
     }
 }
 
 int q4_quantise_launch(const Q4Dims& d, const void* w, int32_t dtype, int64_t ms, int64_t is, int64_t hs, void* rec,
                        int32_t* bad, hipStream_t st) {
-    const int64_t total = (int64_t)d.nm * d.ni * d.nh * d.ngrp;
-    const int64_t wg = (total + Q4_NT - 1) / Q4_NT;
-    const dim3 grid((uint32_t)(wg < 65536 ? wg : 65536));
+    const int64_t rows = (int64_t)d.nm * d.ni;
+    const dim3 grid((uint32_t)(rows < 65536 ? rows : 65536));
     if (dtype == HTM_T_F64)
         hipLaunchKernelGGL(q4_quantise_kernel<double>, grid, dim3(Q4_NT), 0, st, d, (const double*)w, ms, is, hs,
                            (uint8_t*)rec, bad);
@@ -224,6 +239,13 @@ __device__ __forceinline__ void q4_wave_softmax(const float* y, float* q, int nl
 // an even share of the list, its threads the run's blocks side by side, so that
 // a record is read in one piece.  SOFTMAX: the run is whole heads, whose
 // probabilities are written instead.
+//
+// One row is its chain of latencies: pattern, list, records, join, 7 us of 420
+// waves for 1.2 MB.  Rows that share a matrix find it in the caches and are bound by
+// instructions: 4,096 rows of some 600 active cells, 480 outputs, are 4.6e7 wave
+// instructions (2.0 a weight, of which the mask, shift and FMA 1.6), 75 us of
+// issue, in 97 us.  Rows of their own matrices are bound by memory: 256 rows, 7 x
+// 480 outputs, 295 MB in 84 us, 3.5 TB/s.
 template <bool SOFTMAX>
 __global__ void __launch_bounds__(1024) q4_rows_kernel(Q4Dims d, const uint8_t* __restrict__ rec,
                                                        const uint32_t* __restrict__ pat, int64_t ps, int per_model,
@@ -337,7 +359,8 @@ __global__ void __launch_bounds__(1024) q4_rows_kernel(Q4Dims d, const uint8_t* 
         q4_wave_softmax(y_sh + hh * stride, o + (b0 / d.nblk + hh) * d.no, nl, d.no, lane);
 }
 
-// The softmax alone, in place: a wave per (row, head).
+// The softmax alone, in place: a wave per (row, head); 64 rows of 1,000 4 us, one
+// wave's chain, behind products of 15 us.
 __global__ void __launch_bounds__(Q4_NT) q4_softmax_kernel(Q4Dims d, const int32_t* __restrict__ live, int per_model,
                                                            int64_t total, float* __restrict__ y) {
     const int64_t k = (int64_t)blockIdx.x * (Q4_NT / 64) + (threadIdx.x >> 6);
@@ -355,7 +378,9 @@ __global__ void __launch_bounds__(Q4_NT) q4_softmax_kernel(Q4Dims d, const int32
 // exponent under which they count ones (1024 + code, or 64 + code), and a packed
 // subtraction leaves code - 8, exactly: a weight takes part as the number it
 // stands for, with no correction behind the sum, at one instruction more per two
-// weights and rows.
+// weights and rows.  2,048 column confidences, 6 % of them not zero, to 480: 5.5 us,
+// one workgroup's chain; 24,576 numbers to 7 x 480: 22 us for 47 MB, of which the
+// weights' 3.5 instructions are half.
 #define MV_NT 256
 #define MV_HB 16     // outputs of a half block
 
@@ -529,6 +554,12 @@ __global__ void __launch_bounds__(MV_NT, NX == 4 ? 3 : 4)
 // take 32 of the list in turn.  Lane l loads inputs (l / 16) * 8 .. + 7 of half
 // block l % 16, which are B for each of the half block's 16 outputs: 16 sums of
 // [16 rows x 16 half blocks], one for each output of a half block.
+//
+// 8 rows of 24,576 bfloat16 to 7 x 480: 31 us and 5 us for the join (47 MB: 10 us).  8.3e6
+// wave instructions are 14 us of issue, the matrix instructions 3 us beside them;
+// the waves wait 45 % of their time, for records and at the two barriers of a tile, and
+// two workgroups a CU do not cover it.  Reading a step's records one step ahead
+// takes 40 registers and a third workgroup's room: 33 us.
 #define MM_NT 256
 #define MM_ROWS 16
 #define MM_TILE 256
@@ -703,7 +734,8 @@ __global__ void __launch_bounds__(MM_NT, 2)
 }
 
 // The ranges' sums added up: 64 outputs a workgroup, a quarter of the ranges a
-// wave, in a fixed order.
+// wave, in a fixed order.  32 ranges of 8 x 7 x 480: 4.8 us, the latency of eight
+// loads.
 __global__ void __launch_bounds__(256) q4_join_kernel(const float* __restrict__ part, int splits, int64_t n,
                                                       float* __restrict__ out) {
     __shared__ float sm[4][64];
