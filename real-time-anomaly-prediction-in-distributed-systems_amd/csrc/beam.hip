@@ -599,7 +599,7 @@ __global__ void __launch_bounds__(256) rows_copy_kernel(MoveArgs a) {
 // parents' and only then writes, so that no other thread's data is involved and
 // nothing is kept beside the buffers.  Rows that stay are not touched.  The same rows
 // as above, only those that move written: 2 beams 115 us, 8 92 us (5.4 TB/s), 16 103
-// us, 32 139 us, 64 187 us (2.8 TB/s): the more rows a thread holds, the fewer waves
+// us, 32 126 us, 64 187 us (2.8 TB/s): the more rows a thread holds, the fewer waves
 // a CU does.
 template <typename U, int W>
 __device__ __forceinline__ void move_in(const MoveArgs& a, int k, uint32_t block) {
@@ -627,10 +627,10 @@ __device__ __forceinline__ void move_in(const MoveArgs& a, int k, uint32_t block
 }
 
 template <int W>
-__global__ void __launch_bounds__(256, W <= 8 ? 8 : W <= 16 ? 5 : W <= 32 ? 3 : 2) rows_inplace_kernel(MoveArgs a) {
+__global__ void __launch_bounds__(256, W <= 8 ? 8 : W <= 32 ? 5 : 2) rows_inplace_kernel(MoveArgs a) {
     const int k = move_buffer(a);
     const uint32_t b = blockIdx.x - a.first[k];
-    if (W <= 32 && a.width[k] == 4) move_in<unit16, (W <= 32 ? W : 1)>(a, k, b);
+    if (W <= 16 && a.width[k] == 4) move_in<unit16, (W <= 16 ? W : 1)>(a, k, b);
     else if (a.width[k] == 3) move_in<unit8, W>(a, k, b);
     else if (a.width[k] == 2) move_in<uint32_t, W>(a, k, b);
     else if (a.width[k] == 1) move_in<uint16_t, W>(a, k, b);
@@ -655,8 +655,8 @@ int rows_move(const RowMoves& m, const int32_t* idx, int64_t n_rows, int32_t bea
             a.m.dst[i] = m.dst[k];
             a.m.bytes[i] = m.bytes[k];
             const uint64_t all = m.bytes[k] | (uint64_t)(uintptr_t)m.src[k] | (uint64_t)(uintptr_t)m.dst[k];
-            // (64 beams in place: 8-byte units keep a thread's rows in 128 registers)
-            int width = inplace && beams > 32 ? 3 : 4;
+            // (more than 16 beams in place: 8-byte units halve a thread's registers; 32 beams 126 us, by 16 bytes 139)
+            int width = inplace && beams > 16 ? 3 : 4;
             while (width && all & ((1ull << width) - 1)) width--;
             const uint64_t units = m.bytes[k] >> width, per = inplace ? 1 : MOVE_UNITS;
             int lanes = 0;

@@ -4,9 +4,9 @@ against float64 sums of the same weights.
 Tolerance: a weight s * (c - 8) is exact in float32 (8 + 4 bits); a product
 with x rounds once and a sum of n terms n times at most, in whatever order, so
 |y - y64| <= (n + 2) * 2^-24 * sum |x w| per output.  matvec of five and more rows
-a matrix adds up to six exact products a weight instead, whose absolute values sum
-to less than 1 + 2^-6 times |x w|: what can be proved for any order is 6 n in place
-of n.  logits and
+a matrix adds up to six exact products a weight instead, all of one sign, so that
+their absolute values sum to |x w|: what can be proved for any order is 6 n in
+place of n.  logits and
 probabilities sum s * c and take 8 * sum s off at the end: what can be proved
 has sum s (c + 8) in place of sum |x w|.  All are held to the first bound here,
 since so many roundings do not all fall to one side.  softmax: an error d of
