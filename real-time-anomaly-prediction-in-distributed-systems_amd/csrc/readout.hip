@@ -447,24 +447,28 @@ __global__ void __launch_bounds__(MV_NT, NX == 4 ? 3 : 4)
     for (int r = 0; r < NX; r++)
 #pragma unroll
         for (int j = 0; j < MV_HB; j++) a.v[r][j] = 0.0f;
-    float mine[KPT][NX];  // inputs t0 + i * MV_NT + thread
+    T next[KPT][NX];  // inputs t0 + i * MV_NT + thread; as they are: a conversion would wait for them
     auto fetch = [&](int t0) {
 #pragma unroll
         for (int i = 0; i < KPT; i++) {
             const int k = t0 + i * MV_NT + (int)threadIdx.x;
 #pragma unroll
-            for (int r = 0; r < NX; r++) mine[i][r] = k < k1 && r < nx ? x_up(x[(row + r) * xs + k]) : 0.0f;
+            for (int r = 0; r < NX; r++) next[i][r] = k < k1 && r < nx ? x[(row + r) * xs + k] : T(0.0f);
         }
     };
     fetch(k0);
     for (int t0 = k0; t0 < k1; t0 += TILE) {
         uint64_t bal[KPT];
         uint32_t cnt = 0;
+        float mine[KPT][NX];
 #pragma unroll
         for (int i = 0; i < KPT; i++) {
             bool some = false;
 #pragma unroll
-            for (int r = 0; r < NX; r++) some |= mine[i][r] != 0.0f;
+            for (int r = 0; r < NX; r++) {
+                mine[i][r] = x_up(next[i][r]);
+                some |= mine[i][r] != 0.0f;
+            }
             bal[i] = __ballot(some);
             cnt += (uint32_t)__popcll(bal[i]);
         }
@@ -549,21 +553,23 @@ __global__ void __launch_bounds__(MV_NT, NX == 4 ? 3 : 4)
 // float32's normal numbers as zero: scales are kept off that range, and of x and the
 // products 2^-126 may be lost.
 //
-// One workgroup per (16 rows of one matrix, 16 half blocks, range of inputs).  The
-// tile's inputs are listed as above, with their numbers' parts in LDS; its waves
-// take 32 of the list in turn.  Lane l loads inputs (l / 16) * 8 .. + 7 of half
-// block l % 16, which are B for each of the half block's 16 outputs: 16 sums of
-// [16 rows x 16 half blocks], one for each output of a half block.
+// One workgroup per (16 rows of one matrix, 16 half blocks, range of inputs).  A wave
+// takes every fourth 64 inputs of the range for itself: those that are not zero in
+// every row are listed in a ring in LDS with their numbers' parts, and whenever the
+// ring holds 32, they are a step: lane l loads inputs (l / 16) * 8 .. + 7 of half block
+// l % 16, which are B for each of the half block's 16 outputs: 16 sums of [16 rows x
+// 16 half blocks], one for each output of a half block.
 //
-// 8 rows of 24,576 bfloat16 to 7 x 480: 31 us and 5 us for the join (47 MB: 10 us).  8.3e6
-// wave instructions are 14 us of issue, the matrix instructions 3 us beside them;
-// the waves wait 45 % of their time, for records and at the two barriers of a tile, and
-// two workgroups a CU do not cover it.  Reading a step's records one step ahead
-// takes 40 registers and a third workgroup's room: 33 us.
+// 8 rows of 24,576 bfloat16 to 7 x 480: 25 us and 5 us for the join (47 MB: 10 us),
+// bound by instructions: 8.2e6 of a wave, 4.6 a weight and lane, at the 5 cycles each
+// that one or two waves a SIMD reach, are 18 us, the matrix instructions 3, the first
+// records and the waves' join the rest.  A list for the whole workgroup, with barriers:
+// 31 us; registers for three waves a SIMD spill: 47.  A wave's next numbers are read
+// while it works; kept as they are, since a conversion waits for them at once: 30 us.
 #define MM_NT 256
 #define MM_ROWS 16
-#define MM_TILE 256
-#define MM_PITCH (MM_TILE + 8)   // bfloat16 of a row in LDS: 16-byte reads of 16 rows fall on different banks
+#define MM_RING 64               // listed inputs of a wave: less than 32 left over and 32 new ones
+#define MM_PITCH (MM_RING + 8)   // bfloat16 of a row in LDS: 16-byte reads of 16 rows fall on different banks
 #define MM_COLS 272              // floats of a row in the join: 16 x 17
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -574,21 +580,31 @@ template <typename T> struct MmParts { static constexpr int n = 3; };
 template <> struct MmParts<__half> { static constexpr int n = 2; };
 template <> struct MmParts<__hip_bfloat16> { static constexpr int n = 1; };
 
+// LDS that a wave's lanes write for each other: in order for the compiler too
+__device__ __forceinline__ void wave_lds() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+__device__ __forceinline__ f32x4 mm(bf16x8 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(MM_NT, 2)
     q4_mfma_kernel(Q4Dims d, const uint8_t* __restrict__ rec, const T* __restrict__ x, int64_t xs, int per, int y0,
                    int passes, int tiles, int range, float* __restrict__ out, int64_t split_stride) {
     constexpr int P = MmParts<T>::n;
     extern __shared__ __attribute__((aligned(16))) uint8_t mm_sh[];
-    __shared__ uint32_t list[MM_TILE + 32];
-    __shared__ uint32_t wsum[MM_NT / 64];
-    uint16_t* xa = reinterpret_cast<uint16_t*>(mm_sh);  // [P][MM_ROWS][MM_PITCH]
+    __shared__ uint32_t lists[MM_NT / 64][MM_RING];
     const int splits = gridDim.x / tiles, split = blockIdx.x % splits, tile = blockIdx.x / splits;
     const int y = y0 + blockIdx.y, model = y / passes, q0 = (y - model * passes) * MM_ROWS;
     const int nx = min(MM_ROWS, per - q0);
     const int64_t row = (int64_t)model * per + q0;
     const int halves = d.nh * d.nblk * 2;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    uint16_t* xa = reinterpret_cast<uint16_t*>(mm_sh) + wave * (P * MM_ROWS * MM_PITCH);  // [P][MM_ROWS][MM_PITCH]
+    uint32_t* list = lists[wave];
     const int hb = min(tile * 16 + (lane & 15), halves - 1);  // (behind the last: computed again and not written)
     const uint8_t* base = rec + (int64_t)model * d.ni * d.pitch;
     const int h = hb / (d.nblk * 2);
@@ -600,116 +616,127 @@ __global__ void __launch_bounds__(MM_NT, 2)
     f32x4 acc[MV_HB];
 #pragma unroll
     for (int j = 0; j < MV_HB; j++) acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float mine[MM_ROWS];
-    auto fetch = [&](int t0) {
-        const int k = t0 + (int)threadIdx.x;
+    T next[MM_ROWS / 2];  // of input lane % 32, rows r0 .. + 7; as they are: a conversion would wait for them
+    const int r0 = (lane >> 5) * (MM_ROWS / 2), nr = nx - r0;
+    const T* xr = x + (row + r0) * xs + (lane & 31);
+    auto fetch = [&](int t) {
+        const bool in = t + (lane & 31) < k1;
 #pragma unroll
-        for (int r = 0; r < MM_ROWS; r++) mine[r] = k < k1 && r < nx ? x_up(x[(row + r) * xs + k]) : 0.0f;
+        for (int r = 0; r < MM_ROWS / 2; r++) next[r] = in && r < nr ? xr[r * xs + t] : T(0.0f);
     };
-    fetch(k0);
-    for (int t0 = k0; t0 < k1; t0 += MM_TILE) {
-        bool some = false, odd = false;
+    int head = 0, have = 0;  // the ring's first listed input and how many there are
+    bool wild = false;       // an infinity or a NaN among them, or before
+    const auto step = [&](int q) {
+        const int q8 = q + (lane >> 4) * 8;
+        uint2 c[8];
+        uint32_t sc[8];
 #pragma unroll
-        for (int r = 0; r < MM_ROWS; r++) {
+        for (int r = 0; r < 8; r++) {
+            const uint64_t o = (uint64_t)list[q8 + r] << 6;
+            c[r] = *reinterpret_cast<const uint2*>(cbase + o);
+            sc[r] = *reinterpret_cast<const uint16_t*>(sbase + o);
+        }
+        bf16x8 a[P];
+#pragma unroll
+        for (int p = 0; p < P; p++)
+            a[p] = *reinterpret_cast<const bf16x8*>(xa + (p * MM_ROWS + (lane & 15)) * MM_PITCH + q8);
+        __builtin_amdgcn_sched_barrier(0);  // (every load is under way before the first is waited for)
+        // (the scale's lower part may be zero where the weight is not: infinity meets the upper one alone)
+        u32x4 fin = __builtin_bit_cast(u32x4, a[0]);
+        if (wild) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if ((fin[k] & 0x7F80u) == 0x7F80u) fin[k] &= 0xFFFF0000u;
+                if ((fin[k] & 0x7F800000u) == 0x7F800000u) fin[k] &= 0x0000FFFFu;
+            }
+        }
+        const bf16x8 a0 = __builtin_bit_cast(bf16x8, fin);
+        float hi[8], lo[8];
+#pragma unroll
+        for (int r = 0; r < 8; r++) {
+            hi[r] = bf16_up(sc[r] & 0xFFF0u);
+            lo[r] = bf16_up(sc[r]) - hi[r];
+        }
+#pragma unroll
+        for (int g = 0; g < 4; g++) {  // four outputs: half a word of each input's codes
+            uint32_t w[4];
+#pragma unroll
+            for (int p = 0; p < 4; p++)
+                w[p] = __builtin_amdgcn_perm(g < 2 ? c[2 * p + 1].x : c[2 * p + 1].y, g < 2 ? c[2 * p].x : c[2 * p].y,
+                                             g & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                const half2_t bias = n & 1 ? half2_t{(_Float16)72.0f, (_Float16)72.0f}
+                                           : half2_t{(_Float16)1032.0f, (_Float16)1032.0f};
+                u32x4 bh, bl;
+#pragma unroll
+                for (int p = 0; p < 4; p++) {
+                    const uint32_t u = n < 2 ? w[p] : w[p] >> 8;
+                    const half2_t q2 = as_half2(n & 1 ? and_or(u, 0x00F000F0u, e72) : and_or(u, 0x000F000Fu, e1032)) - bias;
+                    const float h0 = __builtin_fmaf((float)q2.x, hi[2 * p], 0.0f);
+                    const float h1 = __builtin_fmaf((float)q2.y, hi[2 * p + 1], 0.0f);
+                    const float l0 = __builtin_fmaf((float)q2.x, lo[2 * p], 0.0f);
+                    const float l1 = __builtin_fmaf((float)q2.y, lo[2 * p + 1], 0.0f);
+                    bh[p] = __builtin_amdgcn_perm(__float_as_uint(h1), __float_as_uint(h0), 0x07060302u);
+                    bl[p] = __builtin_amdgcn_perm(__float_as_uint(l1), __float_as_uint(l0), 0x07060302u);
+                }
+                const int j = g * 4 + n;
+#pragma unroll
+                for (int p = 0; p < P; p++) {
+                    acc[j] = mm(p ? a[p] : a0, bl, acc[j]);
+                    acc[j] = mm(a[p], bh, acc[j]);
+                }
+            }
+        }
+    };
+    fetch(k0 + wave * 32);
+    for (int t = k0 + wave * 32; t < k1; t += MM_NT / 2) {
+        bool some = false, odd = false;
+        float mine[MM_ROWS / 2];
+#pragma unroll
+        for (int r = 0; r < MM_ROWS / 2; r++) {
+            mine[r] = x_up(next[r]);
             some |= mine[r] != 0.0f;
             odd |= !(fabsf(mine[r]) < INFINITY);
         }
-        const uint64_t bal = __ballot(some), odds = __ballot(odd);
-        if (lane == 0) wsum[wave] = (uint32_t)__popcll(bal) | (odds ? 0x10000u : 0u);
-        __syncthreads();
-        uint32_t at = (uint32_t)__popcll(bal & ((1ull << lane) - 1ull)), m = 0;
+        const uint64_t both = __ballot(some);
+        const uint32_t bal = (uint32_t)both | (uint32_t)(both >> 32);
+        wild |= __ballot(odd) != 0;
+        const int at = (head + have + __popc(bal & ((1u << (lane & 31)) - 1u))) & (MM_RING - 1);
+        if ((bal >> (lane & 31)) & 1) {
+            list[at] = (uint32_t)(t + (lane & 31)) * pitch64;
+            uint16_t* to = xa + r0 * MM_PITCH + at;
 #pragma unroll
-        for (int k = 0; k < MM_NT / 64; k++) {
-            const uint32_t c = wsum[k];
-            if (k < wave) at += c & 0xFFFFu;
-            m += c;
-        }
-        const bool wild = m > 0xFFFFu;  // an infinity or a NaN among the tile's numbers
-        m &= 0xFFFFu;
-        // up to a multiple of 32 behind the list: the tile's first input, times zero
-        const uint32_t pad = (32u - (m & 31u)) & 31u;
-        const bool fill = threadIdx.x < pad;
-        if (some) list[at] = (uint32_t)(t0 + (int)threadIdx.x) * pitch64;
-        if (fill) list[m + threadIdx.x] = (uint32_t)t0 * pitch64;
+            for (int r = 0; r < MM_ROWS / 2; r++) {
+                if (r >= nr) break;  // (what the missing rows' lanes read is their own rows' affair, and not written)
+                float v = mine[r];
 #pragma unroll
-        for (int r = 0; r < MM_ROWS; r++) {
-            float v = mine[r];
-#pragma unroll
-            for (int p = 0; p < P; p++) {
-                uint32_t u = __float_as_uint(v) & 0xFFFF0000u;
-                if (v != v) u = 0x7FC00000u;
-                // (what is left of an infinity or a NaN is not a part)
-                v = fabsf(v) < INFINITY ? v - __uint_as_float(u) : 0.0f;
-                if (some) xa[(p * MM_ROWS + r) * MM_PITCH + at] = (uint16_t)(u >> 16);
-                if (fill) xa[(p * MM_ROWS + r) * MM_PITCH + m + threadIdx.x] = 0;
-            }
-        }
-        __syncthreads();
-        fetch(t0 + MM_TILE);  // (the next tile's numbers meanwhile)
-        for (int q = wave * 32; q < (int)m; q += MM_NT / 2) {
-            const int q8 = q + (lane >> 4) * 8;
-            uint2 c[8];
-            uint32_t sc[8];
-#pragma unroll
-            for (int r = 0; r < 8; r++) {
-                const uint64_t o = (uint64_t)list[q8 + r] << 6;
-                c[r] = *reinterpret_cast<const uint2*>(cbase + o);
-                sc[r] = *reinterpret_cast<const uint16_t*>(sbase + o);
-            }
-            bf16x8 a[P];
-#pragma unroll
-            for (int p = 0; p < P; p++)
-                a[p] = *reinterpret_cast<const bf16x8*>(xa + (p * MM_ROWS + (lane & 15)) * MM_PITCH + q8);
-            __builtin_amdgcn_sched_barrier(0);  // (every load is under way before the first is waited for)
-            // (the scale's lower part may be zero where the weight is not: infinity meets the upper one alone)
-            u32x4 fin = __builtin_bit_cast(u32x4, a[0]);
-            if (wild) {
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    if ((fin[k] & 0x7F80u) == 0x7F80u) fin[k] &= 0xFFFF0000u;
-                    if ((fin[k] & 0x7F800000u) == 0x7F800000u) fin[k] &= 0x0000FFFFu;
-                }
-            }
-            const bf16x8 a0 = __builtin_bit_cast(bf16x8, fin);
-            float hi[8], lo[8];
-#pragma unroll
-            for (int r = 0; r < 8; r++) {
-                hi[r] = bf16_up(sc[r] & 0xFFF0u);
-                lo[r] = bf16_up(sc[r]) - hi[r];
-            }
-#pragma unroll
-            for (int g = 0; g < 4; g++) {  // four outputs: half a word of each input's codes
-                uint32_t w[4];
-#pragma unroll
-                for (int p = 0; p < 4; p++)
-                    w[p] = __builtin_amdgcn_perm(g < 2 ? c[2 * p + 1].x : c[2 * p + 1].y, g < 2 ? c[2 * p].x : c[2 * p].y,
-                                                 g & 1 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-                for (int n = 0; n < 4; n++) {
-                    const half2_t bias = n & 1 ? half2_t{(_Float16)72.0f, (_Float16)72.0f}
-                                               : half2_t{(_Float16)1032.0f, (_Float16)1032.0f};
-                    u32x4 bh, bl;
-#pragma unroll
-                    for (int p = 0; p < 4; p++) {
-                        const uint32_t u = n < 2 ? w[p] : w[p] >> 8;
-                        const half2_t q2 = as_half2(n & 1 ? and_or(u, 0x00F000F0u, e72) : and_or(u, 0x000F000Fu, e1032)) - bias;
-                        const float h0 = __builtin_fmaf((float)q2.x, hi[2 * p], 0.0f);
-                        const float h1 = __builtin_fmaf((float)q2.y, hi[2 * p + 1], 0.0f);
-                        const float l0 = __builtin_fmaf((float)q2.x, lo[2 * p], 0.0f);
-                        const float l1 = __builtin_fmaf((float)q2.y, lo[2 * p + 1], 0.0f);
-                        bh[p] = __builtin_amdgcn_perm(__float_as_uint(h1), __float_as_uint(h0), 0x07060302u);
-                        bl[p] = __builtin_amdgcn_perm(__float_as_uint(l1), __float_as_uint(l0), 0x07060302u);
-                    }
-                    const int j = g * 4 + n;
-#pragma unroll
-                    for (int p = 0; p < P; p++) {
-                        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(p ? a[p] : a0, __builtin_bit_cast(bf16x8, bl), acc[j], 0, 0,
-                                                                         0);
-                        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[p], __builtin_bit_cast(bf16x8, bh), acc[j], 0, 0, 0);
-                    }
+                for (int p = 0; p < P; p++) {
+                    uint32_t u = __float_as_uint(v) & 0xFFFF0000u;
+                    if (v != v) u = 0x7FC00000u;
+                    // (what is left of an infinity or a NaN is not a part)
+                    v = fabsf(v) < INFINITY ? v - __uint_as_float(u) : 0.0f;
+                    to[(p * MM_ROWS + r) * MM_PITCH] = (uint16_t)(u >> 16);
                 }
             }
         }
+        have += __popc(bal);
+        fetch(t + MM_NT / 2);  // (the next numbers meanwhile)
+        wave_lds();
+        if (have >= 32) {
+            step(head);
+            head ^= 32;
+            have -= 32;
+        }
+        wave_lds();
+    }
+    if (have) {  // up to 32 behind the list: the range's first input, times zero
+        if (lane >= have && lane < 32) {
+            list[head + lane] = (uint32_t)k0 * pitch64;
+            for (int r = 0; r < P * MM_ROWS; r++) xa[r * MM_PITCH + head + lane] = 0;
+        }
+        wave_lds();
+        step(head);
     }
     // the four waves' sums
     __syncthreads();
@@ -820,13 +847,14 @@ static int q4_raise_lds(const void* kernel, size_t lds, std::atomic<uint64_t>& r
 // How a product is shared out: rows at a time, runs of half blocks and ranges of
 // inputs, some 512 workgroups in all.  Measured, us, both launches:
 //   rows, inputs, outputs          4 rows a pass   8 rows    matrix instructions
-//   1, 24,576, 7 x 480             22 (one row)              35
-//   4, 24,576, 7 x 480             30                        36
-//   8, 24,576, 7 x 480                             44        36 (bfloat16 34)
-//   16, 24,576, 7 x 480                            69        38
-//   8, 24,576, 480                                 18        15
-//   12, 4,000, 7 x 480                             21        16
-//   8, 1,000, 7 x 500                              16        12 (ranges of 256: 14)
+//   1, 24,576, 7 x 480             21 (one row)              32 (bfloat16 28)
+//   4, 24,576, 7 x 480             29                        32 (bfloat16 28)
+//   5, 24,576, 7 x 480                             43        32 (bfloat16 28)
+//   8, 24,576, 7 x 480                             44        33 (bfloat16 28)
+//   16, 24,576, 7 x 480                            76        35
+//   8, 24,576, 480                                 16        14
+//   12, 4,000, 7 x 480                             22        14
+//   8, 24,576 with 6 % not zero, 7 x 480           14        18
 // and for the first two columns, runs x ranges: 8, 24,576, 7 x 480: 7 x 73 44, 7 x
 // 36 50, 4 x 64 58; 1, 4,000, 480: 2 x 16 9.3, 30 x 1 12.5.  In one launch while a
 // tile holds the inputs: 1, 300, 1,000: 16 x 1 5.7, 4 x 4 7.1; 1, 2,048 with 6 %
@@ -870,7 +898,7 @@ template <typename T>
 static int mv_launch(const MvPlan& p, const Q4Dims& d, const void* rec, const void* x, int64_t xs, int per, float* out,
                       int64_t stride, hipStream_t st) {
     const int64_t all = (int64_t)d.nm * p.passes;
-    const size_t lds = std::max<size_t>((size_t)MmParts<T>::n * MM_ROWS * MM_PITCH * 2,
+    const size_t lds = std::max<size_t>((size_t)(MM_NT / 64) * MmParts<T>::n * MM_ROWS * MM_PITCH * 2,
                                         (size_t)4 * std::min(per, MM_ROWS) * MM_COLS * sizeof(float));
     static std::atomic<uint64_t> raised{0};
     if (p.mfma)
