@@ -231,12 +231,17 @@ __global__ void __launch_bounds__(1024) beam_small_kernel(SelArgs a) {
     const int64_t g = a.g0 + blockIdx.x;
     const int lane = threadIdx.x & 63, w0 = (threadIdx.x >> 6) * R;
     const int n = live_of(a, g);
-    const T* x = (const T*)a.x + g * a.gs + w0 * a.bs + lane;
+    const T* x = (const T*)a.x + g * a.gs;
+    T in[R][E];  // (every read without a branch and a conversion, which would wait for it)
     float v[R][E], m[R];
 #pragma unroll
     for (int r = 0; r < R; r++)
 #pragma unroll
-        for (int e = 0; e < E; e++) v[r][e] = w0 + r < a.win && e * 64 + lane < n ? up(x[r * a.bs + e * 64]) : -INFINITY;
+        for (int e = 0; e < E; e++) in[r][e] = x[min(w0 + r, a.win - 1) * a.bs + min(e * 64 + lane, a.v - 1)];
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int e = 0; e < E; e++) v[r][e] = w0 + r < a.win && e * 64 + lane < n ? up(in[r][e]) : -INFINITY;
     float best = -INFINITY;
     uint32_t at = 0;
 #pragma unroll
@@ -306,16 +311,18 @@ __global__ void __launch_bounds__(1024) beam_select_kernel(SelArgs a, int parts,
     const int step = parts * 64, o0 = part * 64 + lane;
     const int all = a.win * a.v;
     for (int i0 = threadIdx.x; i0 < all; i0 += 16 * blockDim.x) {  // 16 loads of a thread under way at once
-        float v[16];
+        T v[16];
+        bool live[16];
 #pragma unroll
         for (int j = 0; j < 16; j++) {
-            const int i = i0 + j * blockDim.x;
+            const int i = min(i0 + j * (int)blockDim.x, all - 1);
             const int w = a.v == 1 ? i : (int)__umulhi((uint32_t)i, inv_v), o = i - w * a.v;
-            v[j] = i < all && o < n ? up(x[(int64_t)w * a.bs + o]) : -INFINITY;
+            v[j] = x[(int64_t)w * a.bs + o];  // (without a branch and a conversion, which would wait for it)
+            live[j] = o < n;
         }
 #pragma unroll
         for (int j = 0; j < 16; j++)
-            if (i0 + j * (int)blockDim.x < all) cand[i0 + j * blockDim.x] = v[j];
+            if (i0 + j * (int)blockDim.x < all) cand[i0 + j * blockDim.x] = live[j] ? up(v[j]) : -INFINITY;
     }
     __syncthreads();
     // eight of a beam's outputs a lane at a time, -infinity behind the live ones
@@ -415,6 +422,17 @@ struct SelWork {
     int32_t chunks;
 };
 
+// A thread's logits of a chunk, -infinity behind the live ones.  Every read without a
+// branch and a conversion, which would wait for it.
+template <typename T>
+__device__ __forceinline__ void chunk_logits(const T* p, int o0, int n, int all, float (&v)[BS_CHUNK / 256]) {
+    T in[BS_CHUNK / 256];
+#pragma unroll
+    for (int j = 0; j < BS_CHUNK / 256; j++) in[j] = p[min(o0 + j * 256 + (int)threadIdx.x, all - 1)];
+#pragma unroll
+    for (int j = 0; j < BS_CHUNK / 256; j++) v[j] = o0 + j * 256 + (int)threadIdx.x < n ? up(in[j]) : -INFINITY;
+}
+
 template <typename T>
 __global__ void __launch_bounds__(256) beam_sums_kernel(SelArgs a, SelWork k, int64_t row0) {
     __shared__ float tm[4];
@@ -424,11 +442,7 @@ __global__ void __launch_bounds__(256) beam_sums_kernel(SelArgs a, SelWork k, in
     const T* p = (const T*)a.x + g * a.gs + (row - g * a.win) * a.bs;
     float v[BS_CHUNK / 256], m = -INFINITY;
     bool nan = false;
-#pragma unroll
-    for (int j = 0; j < BS_CHUNK / 256; j++) {
-        const int o = o0 + j * 256 + threadIdx.x;
-        v[j] = o < n ? up(p[o]) : -INFINITY;
-    }
+    chunk_logits(p, o0, n, a.v, v);
 #pragma unroll
     for (int j = 0; j < BS_CHUNK / 256; j++) {
         m = fmaxf(m, v[j]);
@@ -465,11 +479,7 @@ __global__ void __launch_bounds__(256) beam_chunk_kernel(SelArgs a, SelWork k, i
     const T* p = (const T*)a.x + g * a.gs + w * a.bs;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     float v[BS_CHUNK / 256];
-#pragma unroll
-    for (int j = 0; j < BS_CHUNK / 256; j++) {
-        const int o = o0 + j * 256 + threadIdx.x;
-        v[j] = o < n ? up(p[o]) : -INFINITY;
-    }
+    chunk_logits(p, o0, n, a.v, v);
     // the beam's largest logit and sum from its chunks'
     const float* top = k.top + row * k.chunks;
     const double* sum = k.sum + row * k.chunks;
@@ -501,8 +511,13 @@ __global__ void __launch_bounds__(256) beam_chunk_kernel(SelArgs a, SelWork k, i
 #pragma unroll
         for (int j = 0; j < BS_CHUNK / 256; j++) f(make_key(score_bits(v[j]), place0 + j * 256 + threadIdx.x));
     };
-    const int taken = top_of(make_key(score_bits(best), at), a.wout, sh, each, [&](int r, uint64_t key) { keys[r] = key; });
-    for (int r = taken + (int)threadIdx.x; r < a.wout; r += 256) keys[r] = 0;
+    // every chunk's ranks begin at another place: the merge's classes then hold all ranks and all beams, and their best
+    // make a floor that few keys reach (in order, with beams alike, nearly all do: 4 groups of 16 x 32,768 -> 16 71 us
+    // instead of 6)
+    const int turn = (int)((w * (int64_t)k.chunks + blockIdx.x) % a.wout);
+    const auto place = [&](int r) { return r + turn < a.wout ? r + turn : r + turn - a.wout; };
+    const int taken = top_of(make_key(score_bits(best), at), a.wout, sh, each, [&](int r, uint64_t key) { keys[place(r)] = key; });
+    for (int r = taken + (int)threadIdx.x; r < a.wout; r += 256) keys[place(r)] = 0;
 }
 
 // The chunks' best of one group: the best of them.
@@ -510,15 +525,16 @@ __global__ void __launch_bounds__(1024) beam_merge_kernel(SelArgs a, SelWork k) 
     __shared__ uint64_t tops[16 * 64], list[1024];
     __shared__ uint32_t count;
     const TopSh sh{tops, list, &count, 1024};
-    const int64_t g = a.g0 + blockIdx.x, n = (int64_t)a.win * k.chunks * a.wout;
+    const int64_t g = a.g0 + blockIdx.x;
+    const uint32_t rows = (uint32_t)a.win * (uint32_t)k.chunks, n = rows * (uint32_t)a.wout;  // (at most 2^24 + 4,096)
     const uint64_t* keys = k.keys + g * n;
     uint64_t best = 0;
 #pragma unroll 4
-    for (int64_t i = threadIdx.x; i < n; i += blockDim.x) best = max_key(best, keys[i]);
+    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) best = max_key(best, keys[i]);
     const auto each = [&](auto f) {
-        for (int64_t i = threadIdx.x; i < n; i += blockDim.x) f(keys[i]);
+        for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) f(keys[i]);
     };
-    put_rest(a, g, top_of(best, a.wout, sh, each, [&](int r, uint64_t key) { put_key(a, g, r, key); }));
+    put_rest(a, g, top_of(best, a.wout, sh, each, [&](int r, uint64_t k) { put_key(a, g, r, k); }));
 }
 
 // ------------------------------------------------------------------- rows
