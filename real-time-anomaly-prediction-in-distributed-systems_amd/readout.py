@@ -5,7 +5,7 @@ The reference's Model 1 reads its classifier once learning is off
 (ML/HTM/NetworkModel.py:40-44,70-97, ML/HTM/NetworkUtils.py:166-184).  The
 classifier here keeps NuPIC's float64 matrices, 660 MB a Model-1 stream; a
 `Readout4` holds the same weights in 4 bits with one bfloat16 scale per group
-of neighbouring buckets (46 MB a stream, or 46 MB for a whole fleet that
+of neighbouring buckets (47 MB a stream, or 47 MB for a whole fleet that
 shares its model) and computes
 
     y[r, h, o] = sum_i x[r, i] * scale[m, i, h, o // group] * (code[m, i, h, o] - 8)
