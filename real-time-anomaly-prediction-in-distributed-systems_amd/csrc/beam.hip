@@ -37,6 +37,13 @@ __device__ __forceinline__ uint64_t make_key(uint32_t bits, uint32_t place) {
     return bits ? ((uint64_t)bits << 32) | (0xFFFFFFFFu - place) : 0;
 }
 
+// a * b + c, c a constant in scalar registers.  (Left to itself the compiler moves
+// every constant into the result's registers first, two instructions more.)
+__device__ __forceinline__ double fma_s(double a, double b, double c) {
+    asm("" : "+s"(c));
+    return fma(a, b, c);
+}
+
 // exp(x - m) for finite m >= x, x = -infinity included (0): 2^t as 2^n 2^f, |f| <=
 // 1/2, the Taylor series of 2^f to degree 10 (remainder (ln 2 / 2)^11 / 11! =
 // 2e-13).  A beam's sum off by that much moves a float32 score over a rounding
@@ -46,15 +53,15 @@ __device__ __forceinline__ double exp_diff(float x, double m) {
     const double t = fmax(((double)x - m) * 1.4426950408889634074, -1100.0);
     const double n = rint(t), f = t - n;
     double p = 7.0549116208011233e-9;       // ln(2)^k / k!, k = 10 ... 1
-    p = fma(p, f, 1.0178086009239699e-7);
-    p = fma(p, f, 1.3215486790144309e-6);
-    p = fma(p, f, 1.5252733804059841e-5);
-    p = fma(p, f, 1.5403530393381610e-4);
-    p = fma(p, f, 1.3333558146428443e-3);
-    p = fma(p, f, 9.6181291076284772e-3);
-    p = fma(p, f, 5.5504108664821580e-2);
-    p = fma(p, f, 2.4022650695910071e-1);
-    p = fma(p, f, 6.9314718055994531e-1);
+    p = fma_s(p, f, 1.0178086009239699e-7);
+    p = fma_s(p, f, 1.3215486790144309e-6);
+    p = fma_s(p, f, 1.5252733804059841e-5);
+    p = fma_s(p, f, 1.5403530393381610e-4);
+    p = fma_s(p, f, 1.3333558146428443e-3);
+    p = fma_s(p, f, 9.6181291076284772e-3);
+    p = fma_s(p, f, 5.5504108664821580e-2);
+    p = fma_s(p, f, 2.4022650695910071e-1);
+    p = fma_s(p, f, 6.9314718055994531e-1);
     p = fma(p, f, 1.0);
     return ldexp(p, (int)n);
 }
