@@ -455,7 +455,8 @@ int htm_cls_import_state(htm_classifier* cls, int32_t region, int32_t stream_beg
  * streams can answer too.
  *   y[r][h][o] = sum_i x[r][i] * scale[m][i][h][o / group] * (code[m][i][h][o] - 8)
  * r = 0..n_rows-1, m = r / (n_rows / n_models): consecutive rows share a matrix
- * (a stream's beams; all rows when n_models is 1).  Sums in float32.
+ * (a stream's beams; all rows when n_models is 1); n_rows is a multiple of n_models, at
+ * most 2,097,120.  Sums in float32.
  * Records: uint8 [n_models][n_inputs][htm_q4_record_bytes], one input's weights:
  * per head the codes of its outputs (padded to a multiple of 32; the lower half
  * of a byte first), then per head ceil(padded / group) scales; padding is

@@ -46,7 +46,7 @@ def test_read_out_arguments_refused(rt):
     p, q = ctypes.c_void_p(64), ctypes.c_void_p(72)
     assert L.htm_q4_logits(None, p, p, 1, 1, p, None) == INV
     for args in ((ref(s), None, p, 1, 1, p), (ref(s), q, p, 1, 1, p), (ref(s), p, None, 1, 1, p), (ref(s), p, p, 1, 1, None),
-                 (ref(s), p, p, 0, 2, p), (ref(s), p, p, 1, -1, p), (ref(odd), p, p, 2, 1, p), (ref(two), p, p, 1, 3, p)):
+                 (ref(s), p, p, 0, 2, p), (ref(s), p, p, 1, -1, p), (ref(s), p, p, 1, 65535 * 32 + 1, p), (ref(odd), p, p, 2, 1, p), (ref(two), p, p, 1, 3, p)):
         assert L.htm_q4_logits(*args, None) == INV
     assert L.htm_q4_logits(ref(s), None, None, 1, 0, None, None) == 0      # no rows: nothing to do
     assert L.htm_q4_probabilities(ref(wide), p, p, 1, None, 1, p, None) == INV

@@ -284,12 +284,13 @@ def test_deterministic_and_on_another_stream(rt):
         assert torch.equal(a, c) and torch.equal(b, d)
 
 
-def test_captured_into_graphs(rt):
+@pytest.mark.parametrize("rows", [1, 4, 6])
+def test_captured_into_graphs(rt, rows):
     """Two graphs of the same read-out, replayed in turn with eager calls between, give the eager results."""
     r, _ = make(rt, 1, 24576, 1, 480, 32)
     rng = np.random.default_rng(8)
-    p = words(rng.random((4, 24576)) < 0.02)
-    x = torch.from_numpy(rng.standard_normal((4, 24576))).to(torch.bfloat16).cuda()
+    p = words(rng.random((rows, 24576)) < 0.02)
+    x = torch.from_numpy(rng.standard_normal((rows, 24576))).to(torch.bfloat16).cuda()
     graphs = []
     side = torch.cuda.Stream()
     with torch.cuda.stream(side):
@@ -301,8 +302,8 @@ def test_captured_into_graphs(rt):
             outs = (r.logits(p), r.probabilities(p), r.matvec(x))
         graphs.append((g, outs))
     for k in range(6):
-        p.copy_(words(rng.random((4, 24576)) < 0.02))
-        x.copy_(torch.from_numpy(rng.standard_normal((4, 24576))))
+        p.copy_(words(rng.random((rows, 24576)) < 0.02))
+        x.copy_(torch.from_numpy(rng.standard_normal((rows, 24576))))
         g, outs = graphs[k % 2]
         g.replay()
         want = (r.logits(p), r.probabilities(p), r.matvec(x))
