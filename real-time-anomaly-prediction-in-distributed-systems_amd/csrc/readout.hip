@@ -428,6 +428,7 @@ __global__ void __launch_bounds__(MV_NT, NX == 4 ? 3 : 4)
     __shared__ __attribute__((aligned(16))) float xv[TILE][NX];
     __shared__ uint32_t wsum[MV_NT / 64];
     __shared__ float sm[MV_HB][MV_NT + 1];
+    __shared__ float sums[MV_NT];
     const int splits = gridDim.x / chunks, split = blockIdx.x % splits, chunk = blockIdx.x / splits;
     const int y = y0 + blockIdx.y, model = y / passes, q0 = (y - model * passes) * NX;
     const int nx = min(NX, per - q0);
@@ -525,6 +526,13 @@ __global__ void __launch_bounds__(MV_NT, NX == 4 ? 3 : 4)
     }
     float* o = out + split * split_stride + row * d.nh * d.no;
     const int nout = nb * MV_HB;
+    const auto put = [&](int r, int k, float y) {
+        const int b = b0 + (k >> 4), hh = b / (d.nblk * 2), j = (b - hh * d.nblk * 2) * MV_HB + (k & 15);
+        if (j < d.no) o[(int64_t)r * d.nh * d.no + hh * d.no + j] = y;
+    };
+    // (few outputs: several threads each take a run of slots, then one adds up theirs)
+    const int parts = max(MV_NT / nout, 1), each = (slots + parts - 1) / parts;
+    const int part = threadIdx.x / nout, out0 = threadIdx.x - part * nout;
 #pragma unroll
     for (int r = 0; r < NX; r++) {
         if (r >= nx) break;
@@ -532,12 +540,24 @@ __global__ void __launch_bounds__(MV_NT, NX == 4 ? 3 : 4)
 #pragma unroll
         for (int j = 0; j < MV_HB; j++) sm[j][threadIdx.x] = a.v[r][j];
         __syncthreads();
-        for (int k = threadIdx.x; k < nout; k += MV_NT) {
-            const float* p = &sm[k & 15][k >> 4];
+        if (parts == 1) {
+            for (int k = threadIdx.x; k < nout; k += MV_NT) {
+                const float* p = &sm[k & 15][k >> 4];
+                float y = 0.0f;
+                for (int s = 0; s < slots; s++) y += p[s * nb];
+                put(r, k, y);
+            }
+        } else {
+            const float* p = &sm[out0 & 15][out0 >> 4];
             float y = 0.0f;
-            for (int s = 0; s < slots; s++) y += p[s * nb];
-            const int b = b0 + (k >> 4), hh = b / (d.nblk * 2), j = (b - hh * d.nblk * 2) * MV_HB + (k & 15);
-            if (j < d.no) o[(int64_t)r * d.nh * d.no + hh * d.no + j] = y;
+            if (part < parts)
+                for (int s = part * each; s < min(slots, part * each + each); s++) y += p[s * nb];
+            sums[threadIdx.x] = y;
+            __syncthreads();
+            if ((int)threadIdx.x < nout) {
+                for (int k = 1; k < parts; k++) y += sums[k * nout + threadIdx.x];
+                put(r, threadIdx.x, y);
+            }
         }
     }
 }
@@ -857,8 +877,10 @@ static int q4_raise_lds(const void* kernel, size_t lds, std::atomic<uint64_t>& r
 //   8, 24,576 with 6 % not zero, 7 x 480           14        18
 // and for the first two columns, runs x ranges: 8, 24,576, 7 x 480: 7 x 73 44, 7 x
 // 36 50, 4 x 64 58; 1, 4,000, 480: 2 x 16 9.3, 30 x 1 12.5.  In one launch while a
-// tile holds the inputs: 1, 300, 1,000: 16 x 1 5.7, 4 x 4 7.1; 1, 2,048 with 6 %
-// not zero, 480: 10 x 1 5.9, 2 x 8 7.0.
+// tile holds the inputs (Python call included; in two it takes 12.4): 1, 2,048, 480 8.8;
+// 2, 1,000, 480 8.5 (2, 2,048 11.6); 4, 500, 480 9.9 (4, 1,000 13.0); 8, 200, 480 10.1
+// (8, 400 15.9).  Matrix instructions with ranges of 128 up to 4,096 inputs: 8, 4,000,
+// 480 12.8, of 256 13.3.
 struct MvPlan {
     bool mfma;
     int nx, passes, cb, chunks, splits, range;
@@ -874,12 +896,12 @@ static MvPlan mv_plan(const Q4Dims& d, int per) {
     p.splits = 1;
     const int64_t few = 512;
     if (p.mfma) {
-        const int64_t most = (d.ni + (d.ni <= 2048 ? 127 : 255)) / (d.ni <= 2048 ? 128 : 256);
+        const int64_t most = d.ni <= 256 ? 1 : (d.ni + (d.ni <= 4096 ? 127 : 255)) / (d.ni <= 4096 ? 128 : 256);
         p.chunks = (halves + 15) / 16;
         p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(few / (p.chunks * y), most));
         // (a range's workgroups on one XCD: their pieces of a record share its lines)
         if (p.splits >= 8) p.splits = p.splits / 8 * 8;
-    } else if ((d.ni <= 256 || (per == 1 && d.ni <= 2048)) && (halves + 3) / 4 * y <= few) {
+    } else if (d.ni <= MV_NT * 8 / p.nx && (halves + 3) / 4 * y <= few) {
         p.chunks = (halves + 3) / 4;
     } else {
         const int64_t most = (d.ni + 255) / 256;
