@@ -956,7 +956,10 @@ static int q4_rows_launch(const Q4Dims& d, const void* rec, const uint32_t* pat,
     const int total = d.nh * d.nblk;
     int cblk;
     if (SOFTMAX) {
-        cblk = d.nblk * std::max(1, std::min(d.nh, 64 / d.nblk));
+        // whole heads, as many as leave the chip's CUs a workgroup each (24,576 inputs, 7 x 480, us: 36 rows 1 head 14.5,
+        // 2 16.1, 4 23.8; 128 rows 30.3, 25.5, 25.3)
+        const int64_t heads = ((int64_t)n_rows * d.nh + 255) / 256;
+        cblk = d.nblk * (int)std::max<int64_t>(1, std::min<int64_t>(heads, std::min(d.nh, 64 / d.nblk)));
     } else {
         int chunks = per == 1 && total <= 512 ? 1 : (total + 63) / 64;
         chunks = std::min(total, std::max(chunks, 256 / n_rows));
@@ -995,9 +998,11 @@ int htm_q4_probabilities(const htm_q4_shape* s, const void* rec, const uint32_t*
         return htm_fail(HTM_E_INVALID, "%s: at most %d outputs a head", __func__, Q4_MAX_SOFTMAX);
     if (!n_rows) return HTM_OK;
     hipStream_t st = (hipStream_t)stream;
-    if ((int64_t)n_rows * d.nh >= 256 || d.nblk == 1) return q4_rows_launch<true>(d, rec, pat, ps, n_rows, per, live, out, st);
-    // too few heads to fill the chip: the products in shorter runs, then the softmax (64 rows of 1,000 outputs: in
-    // one launch 30 us, the products 15.5)
+    if (d.nblk <= 4 || (int64_t)n_rows * d.nh >= (d.nblk <= 16 ? 100 : 256))
+        return q4_rows_launch<true>(d, rec, pat, ps, n_rows, per, live, out, st);
+    // too few heads to fill the chip: the products in shorter runs, then the softmax.  One launch and two, us, Python call
+    // included: 64 rows, 65,536 inputs, 1,000 outputs 29 and 19; 255 rows 31 and 33; 24,576 inputs, 480 outputs, 16 rows
+    // 12.7 and 11.6, 128 rows 12.8 and 13.9; 100 outputs, 4 rows 9.3 and 10.8
     if (int r = q4_rows_launch<false>(d, rec, pat, ps, n_rows, per, nullptr, out, st)) return r;
     const int64_t k = (int64_t)n_rows * d.nh;
     hipLaunchKernelGGL(q4_softmax_kernel, dim3((uint32_t)((k + Q4_NT / 64 - 1) / (Q4_NT / 64))), dim3(Q4_NT), 0, st, d, live,
