@@ -1646,7 +1646,8 @@ int htm_create_fleet(const htm_engine* model, int32_t model_stream, int32_t n_st
 // are shared): what a stream needs to go on as another would have, and what
 // htm_get_output reads.  The packed colConfidence always (the next step reads
 // it wherever its flag word says so, also after it was made dense), the dense
-// one unless a step has left it behind.
+// one unless a step has left it behind.  The headers go apart (below); SpBufs::err
+// stays, as no fleet writes it (its one SP instance is dense and never learns).
 static int stream_rows(const htm_engine* e, RowMoves& m) {
     const DevCfg& d = e->dc;
     m.n = 0;
@@ -1658,18 +1659,50 @@ static int stream_rows(const htm_engine* e, RowMoves& m) {
     };
     for (int id = 1; id <= HTM_ST_COUNT; id++) {
         const Region& r = e->regions[id];
-        if (!r.model && id != HTM_ST_TM_COLCONF) add(r.base, r.per_stream);
+        if (!r.model && id != HTM_ST_TM_COLCONF && id != HTM_ST_TM_HEADER) add(r.base, r.per_stream);
     }
     add(e->tm.colnz, ((size_t)d.nw + 1) * 4);
     add(e->tm.colval, (size_t)d.ncol * 4);
     if (!e->conf_packed) add(e->tm.colconf, (size_t)d.ncol * 4);
     add(e->sp.act, HTM_MAXACT * 2);
     add(e->sp.nact, 4);
-    add(e->sp.err, 4);
     add(e->sp.enc_bucket, 16);
     if (e->keep_overlaps) add(e->sp.overlaps, (size_t)d.ncol * 4);
     if (e->keep_prev) add(e->tm.prev_pred, (size_t)d.ncol);
     return HTM_OK;
+}
+
+// The TM headers move with their streams, but a stream's error flags stay and its
+// parent's are added: a flag says that results of this stream were invalid, which
+// no later state undoes (htm_status reports it, as without the move).  Bound by the
+// launch.
+#define HDR_WORDS ((int)(sizeof(htm_tm_header) / 4))
+#define HDR_ERROR ((int)(offsetof(htm_tm_header, error) / 4))
+
+// one workgroup per group of n_beams headers, read whole before the first is written
+__global__ __launch_bounds__(256) void headers_reorder_kernel(htm_tm_header* hdr, const int32_t* parent, int n_beams) {
+    __shared__ uint32_t old[64 * HDR_WORDS];
+    uint32_t* h = reinterpret_cast<uint32_t*>(hdr + (int64_t)blockIdx.x * n_beams);
+    const int32_t* p = parent + (int64_t)blockIdx.x * n_beams;
+    const int words = n_beams * HDR_WORDS;
+    for (int i = threadIdx.x; i < words; i += blockDim.x) old[i] = h[i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < words; i += blockDim.x) {
+        const int w = i / HDR_WORDS, k = i - w * HDR_WORDS, q = p[w];
+        if (q < 0 || q >= n_beams || q == w) continue;
+        h[i] = old[q * HDR_WORDS + k] | (k == HDR_ERROR ? old[i] : 0u);
+    }
+}
+
+// a thread per word of dst's headers
+__global__ __launch_bounds__(256) void headers_copy_kernel(htm_tm_header* dst, const htm_tm_header* src, const int32_t* index,
+                                                           int n, int n_src) {
+    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, s = i / HDR_WORDS;
+    if (s >= n) return;
+    const int q = index[s], k = (int)(i - s * HDR_WORDS);
+    if (q < 0 || q >= n_src) return;
+    uint32_t* to = reinterpret_cast<uint32_t*>(dst) + i;
+    *to = reinterpret_cast<const uint32_t*>(src + q)[k] | (k == HDR_ERROR ? *to : 0u);
 }
 
 // A flush beside the steps reads its streams' headers: rows move after it.  The
@@ -1688,7 +1721,10 @@ int htm_reorder_streams(htm_engine* e, const int32_t* d_parent, int32_t n_beams,
     if (int r = after_flush(e, (hipStream_t)stream)) return r;
     RowMoves m;
     stream_rows(e, m);
-    return rows_move(m, d_parent, e->n, n_beams, e->n, (hipStream_t)stream);
+    if (int r = rows_move(m, d_parent, e->n, n_beams, e->n, (hipStream_t)stream)) return r;
+    hipLaunchKernelGGL(headers_reorder_kernel, dim3(e->n / n_beams), dim3(256), 0, (hipStream_t)stream, e->tm.hdr, d_parent,
+                       n_beams);
+    return hipGetLastError() == hipSuccess ? HTM_OK : htm_fail(HTM_E_HIP, "header move launch failed");
 }
 
 int htm_copy_streams(htm_engine* dst, htm_engine* src, const int32_t* d_index, void* stream) {
@@ -1710,7 +1746,11 @@ int htm_copy_streams(htm_engine* dst, htm_engine* src, const int32_t* d_index, v
     stream_rows(dst, m);
     stream_rows(src, from);
     for (int k = 0; k < m.n; k++) m.src[k] = from.src[k];
-    return rows_move(m, d_index, dst->n, 0, src->n, st);
+    if (int r = rows_move(m, d_index, dst->n, 0, src->n, st)) return r;
+    const int64_t words = (int64_t)dst->n * HDR_WORDS;
+    hipLaunchKernelGGL(headers_copy_kernel, dim3((uint32_t)((words + 255) / 256)), dim3(256), 0, st, dst->tm.hdr, src->tm.hdr,
+                       d_index, dst->n, src->n);
+    return hipGetLastError() == hipSuccess ? HTM_OK : htm_fail(HTM_E_HIP, "header move launch failed");
 }
 
 int32_t htm_is_fleet(const htm_engine* e) { return e && e->fleet ? 1 : 0; }

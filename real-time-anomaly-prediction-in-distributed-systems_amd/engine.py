@@ -229,7 +229,9 @@ class HTMEngine:
         """Fleets: stream g * beams + w goes on as stream g * beams + parent[g, w]
         would have (parent: int32 device tensor [n_streams / beams, beams], beams
         <= 64; a parent outside 0..beams-1 counts as w).  Every per-stream state
-        and output moves, in place; counters follow the state."""
+        and output moves, in place; counters follow the state.  Error flags
+        stay with their stream and its parent's are added, so that `status`
+        raises for an overflow in a stream whose state has been replaced."""
         if not isinstance(parent, torch.Tensor) or parent.dtype != torch.int32 or parent.dim() != 2 or \
                 parent.device != torch.device("cuda", self.device) or parent.numel() != self.n_streams:
             raise ValueError(f"parent must be int32 [n_streams / beams, beams] on cuda:{self.device}")
@@ -240,7 +242,8 @@ class HTMEngine:
     def copy_streams(self, src: "HTMEngine", index):
         """Fleets of one model: stream s of this engine goes on as stream
         index[s] of `src` (int32 device tensor [n_streams]; an index outside
-        src leaves s as it is) -- the fork of a fleet's streams into beams."""
+        src leaves s as it is) -- the fork of a fleet's streams into beams.
+        Error flags as in `reorder_streams`."""
         if not isinstance(index, torch.Tensor) or index.dtype != torch.int32 or \
                 index.device != torch.device("cuda", self.device) or index.shape != (self.n_streams,):
             raise ValueError(f"index must be int32 [{self.n_streams}] on cuda:{self.device}")

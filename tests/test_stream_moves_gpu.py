@@ -1,0 +1,93 @@
+"""What a move of a fleet's streams must not lose or accept (HTMEngine.reorder_streams, copy_streams,
+harness.model_forecast)."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+if not torch.cuda.is_available():
+    pytest.skip("needs a GPU", allow_module_level=True)
+
+OVERFLOW = 16  # htm_tm_header.error: qualifying-segment list overflow
+
+
+def trained(rt, traces, steps=120, first=0):
+    eng = rt.HTMEngine(1, seg_capacity=1 << 14)
+    for v in traces["train"][first:first + steps]:
+        eng.step(torch.tensor([v], dtype=torch.float64, device="cuda"))
+    return eng
+
+
+@pytest.fixture(scope="module")
+def model(rt, traces):
+    return trained(rt, traces)
+
+
+def flag(rt, fleet, stream, bits):
+    """The stream's header as an overflow leaves it."""
+    h = fleet.tm_header(stream)
+    h.error |= bits
+    fleet.import_state("tm_header", np.frombuffer(bytes(h), np.uint8)[None], stream)
+
+
+def flags(fleet):
+    return [fleet.tm_header(s).error for s in range(fleet.n_streams)]
+
+
+def step(fleet, value):
+    fleet.step(torch.full((fleet.n_streams,), float(value), dtype=torch.float64, device="cuda"))
+
+
+@pytest.mark.parametrize("beams", [1, 3, 6])
+def test_flags_stay_with_a_stream_that_is_reordered(rt, model, beams):
+    fl = rt.HTMEngine.fleet(model, 6, q_capacity=4096)
+    step(fl, 30)
+    flag(rt, fl, 1, OVERFLOW)
+    flag(rt, fl, 5, 2)
+    parent = np.zeros((6 // beams, beams), np.int32)   # the first stream of a group is the parent of all
+    parent[-1, -1] = 99                                # outside: the stream itself
+    fl.reorder_streams(torch.from_numpy(parent).cuda())
+    at = (parent % 99 + np.arange(6 // beams)[:, None] * beams).reshape(-1)
+    old = [0, OVERFLOW, 0, 0, 0, 2]
+    assert flags(fl) == [old[s] | (old[at[s]] if s < 5 else 0) for s in range(6)]
+    with pytest.raises(rt.HtmError, match="q_capacity|queue full"):
+        fl.status()
+    if beams > 1:  # a flagged parent's children are flagged too
+        fl.reorder_streams(torch.full((6 // beams, beams), 1, dtype=torch.int32, device="cuda"))
+        assert flags(fl)[0] == OVERFLOW
+    step(fl, 31)
+    with pytest.raises(rt.HtmError):
+        fl.status()
+
+
+def test_flags_stay_with_a_stream_that_is_copied_to(rt, model):
+    src, dst = rt.HTMEngine.fleet(model, 2, q_capacity=4096), rt.HTMEngine.fleet(model, 5, q_capacity=4096)
+    step(src, 30), step(dst, 40)
+    flag(rt, dst, 3, OVERFLOW)
+    index = torch.tensor([0, 1, -1, 0, 7], dtype=torch.int32, device="cuda")
+    dst.copy_streams(src, index)
+    assert flags(dst) == [0, 0, 0, OVERFLOW, 0] and flags(src) == [0, 0]
+    flag(rt, src, 1, 1)
+    dst.copy_streams(src, index)
+    assert flags(dst) == [0, 1, 0, OVERFLOW, 0]
+    with pytest.raises(rt.HtmError):
+        dst.status()
+
+
+@pytest.mark.parametrize("horizon", [2, 4])
+def test_a_forecast_raises_for_a_beam_that_was_replaced(rt, model, horizon):
+    """An overflow of an early look-ahead step: the beam's state is replaced by forks and reorders many times after."""
+    w = torch.from_numpy(np.random.default_rng(3).standard_normal((1, model.n_columns, 1, 480))).cuda()
+    ro = rt.Readout4.quantize(w)
+    fl, bf = rt.HTMEngine.fleet(model, 2, q_capacity=4096), rt.HTMEngine.fleet(model, 8, q_capacity=4096)
+    records = np.array([20.0, 30.0, 25.0])
+    rt.harness.model_forecast(fl, bf, ro, records, horizon=horizon, source="col_confidence")
+    for stream in (0, 3, 6):
+        flag(rt, bf, stream, OVERFLOW)
+        with pytest.raises(rt.HtmError, match="q_capacity"):
+            rt.harness.model_forecast(fl, bf, ro, records, horizon=horizon, source="col_confidence")
+        for s in range(8):                             # (its children are flagged too)
+            h = bf.tm_header(s)
+            h.error = 0
+            bf.import_state("tm_header", np.frombuffer(bytes(h), np.uint8)[None], s)
+    rt.harness.model_forecast(fl, bf, ro, records, horizon=horizon, source="col_confidence")
