@@ -362,6 +362,10 @@ int htm_replicate_stream(htm_engine* eng, int32_t src, void* stream);
 int htm_create_fleet(const htm_engine* model, int32_t model_stream, int32_t n_streams, int32_t q_capacity,
                      int32_t device, htm_engine** out);
 int32_t htm_is_fleet(const htm_engine* eng);
+/* A number of a fleet's model's contents, alike for fleets of one model (built at any
+ * time, saved and loaded) and, but for a chance of 2^-64, for no others.  Known since
+ * htm_create_fleet / htm_load; counted anew (synchronising) behind htm_import_state. */
+int htm_model_id(htm_engine* eng, uint64_t* out);
 
 /* Engine introspection */
 int32_t htm_n_streams(const htm_engine* eng);
@@ -542,7 +546,8 @@ int htm_reorder_streams(htm_engine* eng, const int32_t* d_parent, int32_t n_beam
 /* Stream s of fleet dst goes on as stream d_index[s] (DEVICE int32 [n_streams of
  * dst], 0..n_streams of src - 1; others leave s as it is) of fleet src: a fork.  Error
  * flags as above.
- * Both are fleets of one model, alike in configuration, on one device; dst != src. */
+ * Both are fleets of one model (htm_model_id) and configuration on one device; others
+ * are refused; dst != src. */
 int htm_copy_streams(htm_engine* dst, htm_engine* src, const int32_t* d_index, void* stream);
 
 const char* htm_last_error(void);

@@ -122,7 +122,7 @@ EXPORTED = [
     "htm_import_state", "htm_reset_tm", "htm_save", "htm_load", "htm_replicate_stream", "htm_n_streams",
     "htm_get_config", "htm_device_bytes", "htm_sp_perm_rows_used", "htm_frozen_index_valid", "htm_last_error", "htm_abi_version",
     "htm_profile_read", "htm_counters", "htm_debug_stamps", "htm_build_info",
-    "htm_slo_create", "htm_slo_destroy", "htm_slo_record", "htm_slo_stats", "htm_create_fleet", "htm_is_fleet", "htm_flush",
+    "htm_slo_create", "htm_slo_destroy", "htm_slo_record", "htm_slo_stats", "htm_create_fleet", "htm_is_fleet", "htm_model_id", "htm_flush",
     "htm_likelihood_create", "htm_likelihood_destroy", "htm_likelihood_step",
     "htm_cls_create", "htm_cls_destroy", "htm_cls_compute", "htm_cls_status", "htm_cls_state_bytes",
     "htm_cls_export_state", "htm_cls_import_state", "htm_cls_quantise",
@@ -231,6 +231,7 @@ def lib():
     L.htm_beam_work_bytes.restype = sz
     L.htm_beam_select.argtypes = [vp, i32, i64, i64, vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, sz, vp]
     L.htm_beam_reorder.argtypes = [i32, vp, vp, vp, vp, i32, i32, vp]
+    L.htm_model_id.argtypes = [vp, P(ctypes.c_uint64)]
     L.htm_reorder_streams.argtypes = [vp, vp, i32, vp]
     L.htm_copy_streams.argtypes = [vp, vp, vp, vp]
     _lib = L

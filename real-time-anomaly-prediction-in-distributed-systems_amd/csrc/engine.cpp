@@ -118,6 +118,8 @@ struct htm_engine {
                                       // 0.1548 -> 0.1529 ms/step same box, profiles/r06_ab/flush_stream/)
     size_t enc_cap = 0;               // steps SpBufs::enc_in holds (RDSE engines)
     bool conf_packed = false;         // a step kernel wrote colConfidence packed since the last densify
+    uint64_t model_id = 0;            // fleets: htm_model_id, while model_id_known
+    bool model_id_known = false;
     bool lp2_pending = false;         // a learning step may have left its final learn phase 2 pending
     int32_t ordered = 1;              // HTM_OPT_ORDERED: frozen lockstep steps run their TM steps heaviest first
     int32_t split_learn = 1;          // HTM_OPT_SPLIT_LEARN: learning lockstep steps run the SP kernel, then TM-only
@@ -1513,6 +1515,7 @@ static int import_region(htm_engine* e, int32_t region, int32_t s0, int32_t n, c
     if (int rf = flush_sync(e)) return rf;
     if (int rd = densify_conf(e, nullptr)) return rd;  // (before the dense copy may be overwritten)
     HIP_TRY(hipDeviceSynchronize());
+    e->model_id_known = false;
     if (region == HTM_ST_SP_PERM && e->dc.sp_paged) return paged_perm_import(e, s0, n, h_src, nullptr, 0);
     if (rebase && e->dc.sp_paged && (region == HTM_ST_SP_PERM_CKPT || region == HTM_ST_SP_POTMASK))
         return paged_rebase_import(e, region, s0, n, h_src);
@@ -1592,6 +1595,58 @@ int htm_replicate_stream(htm_engine* e, int32_t src, void* stream) {
     return HTM_OK;
 }
 
+// Sum over the words of mix(place, word), modulo 2^64: the same in any order.
+__global__ __launch_bounds__(256) void model_hash_kernel(const uint8_t* p, uint64_t bytes, uint64_t seed,
+                                                         unsigned long long* out) {
+    const uint64_t words = (bytes + 3) / 4;
+    uint64_t sum = 0;
+    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < words; i += (uint64_t)gridDim.x * blockDim.x) {
+        uint32_t w = 0;
+        if (i * 4 + 4 <= bytes) w = reinterpret_cast<const uint32_t*>(p)[i];
+        else
+            for (uint64_t k = i * 4; k < bytes; k++) w |= (uint32_t)p[k] << (8 * (k & 3));
+        uint64_t z = (i + 1) * 0x9E3779B97F4A7C15ull + seed;   // two rounds of multiply and xor-shift
+        z = (z ^ (z >> 31) ^ w) * 0xD6E8FEB86659FD93ull;
+        z = (z ^ (z >> 29) ^ ((uint64_t)w << 32)) * 0xA3B195354A39B70Dull;
+        sum += z ^ (z >> 32);
+    }
+    for (int k = 32; k; k >>= 1) sum += __shfl_xor((unsigned long long)sum, k);
+    if ((threadIdx.x & 63) == 0) atomicAdd(out, (unsigned long long)sum);
+}
+
+// What a fleet's streams share and their results rest on.  Steps of a fleet change
+// none of it: of the model's regions they write the dutyCycle records alone, which
+// are left out (as are the SP's duty cycles and the update queue, of learning).
+int htm_model_id(htm_engine* e, uint64_t* out) {
+    if (!e || !out) return htm_fail(HTM_E_INVALID, "bad arguments");
+    if (!e->fleet) return htm_fail(HTM_E_STATE, "an ordinary engine's streams have models of their own");
+    if (!e->model_id_known) {
+        htm_tm_header h;
+        HIP_TRY(hipDeviceSynchronize());
+        HIP_TRY(hipMemcpy(&h, e->tm.hdr, sizeof h, hipMemcpyDeviceToHost));
+        unsigned long long* d = nullptr;
+        unsigned long long x[1] = {((unsigned long long)h.lrn_iter << 32 | h.seg_hwm) * 0x9E3779B97F4A7C15ull + h.seg_live};
+        HIP_TRY(hipMalloc(&d, sizeof x));
+        bool ok = hipMemcpy(d, x, sizeof x, hipMemcpyHostToDevice) == hipSuccess;
+        for (int id : {HTM_ST_SP_CONNT, HTM_ST_SP_POTMASK, HTM_ST_SP_PERM, HTM_ST_SP_BOOST, HTM_ST_TM_SEG_META, HTM_ST_TM_SEG_SRC,
+                       HTM_ST_TM_SEG_PERM, HTM_ST_TM_SEG_CONN, HTM_ST_TM_CELL_NSEG}) {
+            const Region& r = e->regions[id];
+            if (ok && r.base && r.per_stream) {
+                hipLaunchKernelGGL(model_hash_kernel, dim3(1024), dim3(256), 0, nullptr, (const uint8_t*)r.base,
+                                   (uint64_t)r.per_stream, (uint64_t)id << 56, d);
+                ok = hipGetLastError() == hipSuccess;
+            }
+        }
+        ok = ok && hipMemcpy(x, d, sizeof x, hipMemcpyDeviceToHost) == hipSuccess;
+        (void)hipFree(d);
+        if (!ok) return htm_fail(HTM_E_HIP, "model identity: %s", hipGetErrorString(hipGetLastError()));
+        e->model_id = x[0];
+        e->model_id_known = true;
+    }
+    *out = e->model_id;
+    return HTM_OK;
+}
+
 int htm_create_fleet(const htm_engine* model, int32_t model_stream, int32_t n_streams, int32_t q_capacity,
                      int32_t device, htm_engine** out) {
     if (!model || !out || n_streams < 1 || q_capacity < 64) return htm_fail(HTM_E_INVALID, "bad arguments");
@@ -1633,6 +1688,8 @@ int htm_create_fleet(const htm_engine* model, int32_t model_stream, int32_t n_st
                hipMemcpy(e->sp.nact, model->sp.nact + model_stream, 4, hipMemcpyDefault) != hipSuccess))
         r = htm_fail(HTM_E_HIP, "fleet copy of the SP output");
     if (!r) r = htm_replicate_stream(e, 0, nullptr);
+    uint64_t id;
+    if (!r) r = htm_model_id(e, &id);
     if (r) {
         htm_destroy(e);
         return r;
@@ -1733,6 +1790,10 @@ int htm_copy_streams(htm_engine* dst, htm_engine* src, const int32_t* d_index, v
     if (dst->device != src->device) return htm_fail(HTM_E_INVALID, "the fleets are on devices %d and %d", dst->device, src->device);
     if (std::memcmp(&dst->cfg, &src->cfg, sizeof(htm_config)))
         return htm_fail(HTM_E_INVALID, "the fleets' configurations differ");
+    uint64_t a, b;
+    if (int r = htm_model_id(dst, &a)) return r;
+    if (int r = htm_model_id(src, &b)) return r;
+    if (a != b) return htm_fail(HTM_E_INVALID, "the fleets' models differ");
     if (dst->keep_overlaps != src->keep_overlaps || dst->keep_prev != src->keep_prev)
         return htm_fail(HTM_E_INVALID, "the fleets retain different outputs (HTM_OPT_KEEP_*)");
     hipStream_t st = (hipStream_t)stream;
@@ -1901,6 +1962,11 @@ int htm_load(const char* path, int32_t device, htm_engine** out) {
     }
     e->sp_learn = fleet ? 0 : spl;
     e->tm_learn = fleet ? 0 : tml;
+    uint64_t id;
+    if (int ri = fleet ? htm_model_id(e, &id) : HTM_OK) {
+        htm_destroy(e);
+        return ri;
+    }
     *out = e;
     return HTM_OK;
 }

@@ -69,6 +69,13 @@ class HTMEngine:
                                      ctypes.byref(h)))
         return cls(0, device=dev, _handle=h)
 
+    def model_id(self) -> int:
+        """Fleets: a number of the shared model's contents, alike for fleets of one model only."""
+        x = ctypes.c_uint64()
+        with torch.cuda.device(self.device):
+            check(self._L.htm_model_id(self.h, ctypes.byref(x)))
+        return x.value
+
     def _model_index(self, s: int) -> int:
         """instance of the model regions stream s reads (fleet: the shared one)"""
         return 0 if self.is_fleet else s
@@ -243,6 +250,7 @@ class HTMEngine:
         """Fleets of one model: stream s of this engine goes on as stream
         index[s] of `src` (int32 device tensor [n_streams]; an index outside
         src leaves s as it is) -- the fork of a fleet's streams into beams.
+        Fleets of different models (`model_id`) are refused.
         Error flags as in `reorder_streams`."""
         if not isinstance(index, torch.Tensor) or index.dtype != torch.int32 or \
                 index.device != torch.device("cuda", self.device) or index.shape != (self.n_streams,):

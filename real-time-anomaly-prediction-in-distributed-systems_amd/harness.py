@@ -245,6 +245,8 @@ def model_forecast(fleet, beam_fleet, readout, cpu, horizon=LOOKAHEAD, bucket_va
         raise ValueError("the read-out has %d inputs, %s %d" % (readout.n_inputs, source, width))
     if beam_fleet.device != fleet.device or readout.device != torch.device("cuda", fleet.device):
         raise ValueError("the fleets and the read-out must be on one device")
+    if beam_fleet.model_id() != fleet.model_id():
+        raise ValueError("model_forecast needs two fleets of one model: these were built from different ones")
     dev = f"cuda:{fleet.device}"
     c = fleet.config
     if bucket_values is None:

@@ -91,3 +91,56 @@ def test_a_forecast_raises_for_a_beam_that_was_replaced(rt, model, horizon):
             h.error = 0
             bf.import_state("tm_header", np.frombuffer(bytes(h), np.uint8)[None], s)
     rt.harness.model_forecast(fl, bf, ro, records, horizon=horizon, source="col_confidence")
+
+
+def test_fleets_of_different_models_are_refused(rt, model, traces, tmp_path):
+    """Alike in configuration: trained on other records, and one model before and after more training."""
+    index = torch.zeros(3, dtype=torch.int32, device="cuda")
+    other = trained(rt, traces, first=400)
+    grown = trained(rt, traces)
+    early = rt.HTMEngine.fleet(grown, 3, q_capacity=4096)
+    for v in traces["train"][120:150]:
+        grown.step(torch.tensor([v], dtype=torch.float64, device="cuda"))
+    late = rt.HTMEngine.fleet(grown, 3, q_capacity=4096)
+    fl = rt.HTMEngine.fleet(model, 3, q_capacity=4096)
+    for dst, src in ((fl, rt.HTMEngine.fleet(other, 2, q_capacity=4096)), (early, late), (late, early)):
+        assert dst.model_id() != src.model_id()
+        with pytest.raises(rt.HtmError, match="models differ"):
+            dst.copy_streams(src, index)
+    w = torch.from_numpy(np.random.default_rng(3).standard_normal((1, model.n_columns, 1, 480))).cuda()
+    ro = rt.Readout4.quantize(w)
+    step(fl, 10)
+    before = fl.export_state("tm_header")
+    with pytest.raises(ValueError, match="one model"):
+        rt.harness.model_forecast(fl, rt.HTMEngine.fleet(other, 6, q_capacity=4096), ro, np.array([20.0]), horizon=2,
+                                  source="col_confidence")
+    assert np.array_equal(before, fl.export_state("tm_header"))   # refused before the first step
+    with pytest.raises(rt.HtmError):
+        model.model_id()
+
+
+def test_fleets_of_one_model_are_not(rt, model, traces, tmp_path):
+    """Built at different times, with different list capacities, stepped, saved and loaded, from models equal in
+    content: one identity."""
+    index = torch.zeros(3, dtype=torch.int32, device="cuda")
+    a = rt.HTMEngine.fleet(model, 3, q_capacity=4096)
+    for v in (10, 50, 90, 20, 30, 40, 50, 60, 70):
+        step(a, v)                                       # (a flush of the deferred writes among them)
+    a.save(str(tmp_path / "fleet"))
+    loaded = rt.HTMEngine.load(str(tmp_path / "fleet"))
+    again = trained(rt, traces)                          # the same training once more
+    b, c = rt.HTMEngine.fleet(model, 2, q_capacity=2048), rt.HTMEngine.fleet(again, 5, q_capacity=4096)
+    ids = {e.model_id() for e in (a, b, c, loaded)}
+    assert len(ids) == 1
+    for src in (b, c, loaded):
+        a.copy_streams(src, index)
+    # another model's state imported makes another fleet of it, its own makes it this one again
+    own = b.export_state("tm_seg_perm", 0, 1)
+    b.import_state("tm_seg_perm", np.zeros_like(own))
+    assert b.model_id() not in ids
+    with pytest.raises(rt.HtmError, match="models differ"):
+        a.copy_streams(b, index)
+    b.import_state("tm_seg_perm", own)
+    assert b.model_id() in ids
+    a.copy_streams(b, index)
+    a.status()
