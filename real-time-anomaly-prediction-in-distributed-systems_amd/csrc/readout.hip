@@ -20,7 +20,7 @@
 #include "q4_dev.h"
 
 #define Q4_NT 256
-#define Q4_MAX_SCALE 1.2676506002282294e30  // 2^100: a scale times 2^24 stays finite (Q4Acc)
+#define Q4_MAX_SCALE 1.2676506002282294e30  // 2^100: 65,536 weights' sum stays finite
 #define Q4_MIN_SCALE 7.7037197775489434e-34 // 2^-110: its lower four bits are a normal number (q4_mfma_kernel)
 
 int q4_dims(const htm_q4_shape* s, const char* who, Q4Dims* d) {
@@ -125,44 +125,50 @@ int q4_quantise_launch(const Q4Dims& d, const void* w, int32_t dtype, int64_t ms
 }
 
 // ------------------------------------------------------------------ products
-// A record's block: 32 outputs' codes in 16 bytes, under one scale.  A code's
-// four bits lie in the low mantissa bits of a 16-bit float of exponent zero:
-// masked there they are the number code * 2^-24 (bits 0-3) or code * 2^-20
-// (bits 4-7), a subnormal float16 that a mixed-precision FMA reads exactly --
-// one mask and one FMA a weight, 13 instructions per 8 weights with the shift
-// (shift, convert and FMA apart: 24).  The sum of scale * code is corrected by
-// 8 * sum of scales once at the end.
+// A record's block: 32 outputs' codes in 16 bytes, under one scale.  A code's four
+// bits are masked where they lie, under the exponent that makes the lowest of them
+// count one, and a subtraction leaves code - 8, exactly: a weight takes part as the
+// number it stands for (11 bits at most), so that one of zero adds nothing, however
+// large its scale.  Three full-rate instructions a weight, and a shift for eight.
+// Measured, us (4,096 rows of 600 of 24,576 inputs, 480 outputs; 256 rows of own
+// matrices, 7 heads): 108 and 83; by pairs of half floats, a packed subtraction and
+// mixed FMAs 115 and 92; by v_cvt_off_f32_i4 124 and 98.  (Sums of scale * code with 8 *
+// the sum of scales taken off at the end take 95 and 78, but a large scale then rounds
+// the other inputs' weights away.)
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ half2_t as_half2(uint32_t u) { return __builtin_bit_cast(half2_t, u); }
 
+// (a & mask) | bits as one instruction: its operands allow one constant, so the
+// other has to be kept in a register, which the compiler does not do by itself.
+__device__ __forceinline__ uint32_t in_vgpr(uint32_t c) {
+    asm("" : "+v"(c));
+    return c;
+}
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) { return (a & mask) | bits; }
+
 struct Q4Acc {
     float v[Q4_BLK];
-    float s;
     __device__ __forceinline__ void clear() {
 #pragma unroll
         for (int j = 0; j < Q4_BLK; j++) v[j] = 0.0f;
-        s = 0.0f;
     }
-    // + m * (codes), m the scale times the input's number
+    // + m * (codes - 8), m the scale
     __device__ __forceinline__ void add(uint4 c, float m) {
-        const float m0 = m * 16777216.0f, m1 = m * 1048576.0f;
-        s += m;
         const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+        uint32_t e[5];  // 2^(23 - 4 n): bits 4 n and up count ones
+#pragma unroll
+        for (int n = 0; n < 5; n++) e[n] = in_vgpr((uint32_t)(127 + 23 - 4 * n) << 23);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const uint32_t u = w[k], h = w[k] >> 8;
-            const half2_t a = as_half2(u & 0x000F000Fu), b = as_half2(u & 0x00F000F0u);
-            const half2_t d = as_half2(h & 0x000F000Fu), e = as_half2(h & 0x00F000F0u);
+            const uint32_t h = w[k] >> 12;
             float* p = v + k * 8;
-            p[0] = __builtin_fmaf((float)a.x, m0, p[0]);
-            p[1] = __builtin_fmaf((float)b.x, m1, p[1]);
-            p[2] = __builtin_fmaf((float)d.x, m0, p[2]);
-            p[3] = __builtin_fmaf((float)e.x, m1, p[3]);
-            p[4] = __builtin_fmaf((float)a.y, m0, p[4]);
-            p[5] = __builtin_fmaf((float)b.y, m1, p[5]);
-            p[6] = __builtin_fmaf((float)d.y, m0, p[6]);
-            p[7] = __builtin_fmaf((float)e.y, m1, p[7]);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int n = j < 5 ? j : j - 3;
+                const float x = __uint_as_float(and_or(j < 5 ? w[k] : h, 0xFu << (4 * n), e[n]));
+                p[j] = __builtin_fmaf(x - ((float)(1u << (23 - 4 * n)) + 8.0f), m, p[j]);
+            }
         }
     }
 };
@@ -175,12 +181,11 @@ template <typename PUT>
 __device__ __forceinline__ void q4_join(Q4Acc& a, int nblk, int slots, float* sm, PUT put) {
     const int nt = blockDim.x, nout = nblk * 16;
     const int parts = nout < nt ? nt / nout : 1;
-    const float off = 8.0f * a.s;
 #pragma unroll
     for (int half = 0; half < 2; half++) {
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < 16; j++) sm[j * (nt + 1) + threadIdx.x] = a.v[half * 16 + j] - off;
+        for (int j = 0; j < 16; j++) sm[j * (nt + 1) + threadIdx.x] = a.v[half * 16 + j];
         __syncthreads();
         if (parts == 1) {
             for (int o = threadIdx.x; o < nout; o += nt) {
@@ -242,10 +247,13 @@ __device__ __forceinline__ void q4_wave_softmax(const float* y, float* q, int nl
 //
 // One row is its chain of latencies: pattern, list, records, join, 7 us of 420
 // waves for 1.2 MB.  Rows that share a matrix find it in the caches and are bound by
-// instructions: 4,096 rows of some 600 active cells, 480 outputs, are 4.6e7 wave
-// instructions (2.0 a weight, of which the mask, shift and FMA 1.6), 75 us of
-// issue, in 97 us.  Rows of their own matrices are bound by memory: 256 rows, 7 x
-// 480 outputs, 295 MB in 84 us, 3.5 TB/s.
+// instructions: 4,096 rows of 768 columns x 32 cells, some 600 of them active, 480
+// outputs, are 7.2e7 wave instructions (3.9 a weight, of which mask, subtraction,
+// FMA and shift 3.1), 75 us of issue at 2.5 cycles each, in 108 us; of 2,048 x 12, 280
+// active, 58 us.  Rows of their own matrices (256 rows, 7 x 480 outputs, 295 MB in 83
+// us; of 2,048 x 12 37) are bound by what one workgroup moves and unpacks: the 40 % of
+// the rows whose columns burst, 1,280 cells each, hold 85 % of the bytes, and some 100
+// workgroups work on while the others have ended.
 template <bool SOFTMAX>
 __global__ void __launch_bounds__(1024) q4_rows_kernel(Q4Dims d, const uint8_t* __restrict__ rec,
                                                        const uint32_t* __restrict__ pat, int64_t ps, int per_model,
@@ -383,14 +391,6 @@ __global__ void __launch_bounds__(Q4_NT) q4_softmax_kernel(Q4Dims d, const int32
 // weights' 3.5 instructions are half.
 #define MV_NT 256
 #define MV_HB 16     // outputs of a half block
-
-// (a & mask) | bits as one instruction: its operands allow one constant, so the
-// other has to be kept in a register, which the compiler does not do by itself.
-__device__ __forceinline__ uint32_t in_vgpr(uint32_t c) {
-    asm("" : "+v"(c));
-    return c;
-}
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) { return (a & mask) | bits; }
 
 template <int NX>
 struct MvAcc {
