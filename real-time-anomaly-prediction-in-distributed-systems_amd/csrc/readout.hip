@@ -385,10 +385,9 @@ __global__ void __launch_bounds__(Q4_NT) q4_softmax_kernel(Q4Dims d, const int32
 // a weight is read and unpacked once for all of them.  Here a code's bits get the
 // exponent under which they count ones (1024 + code, or 64 + code), and a packed
 // subtraction leaves code - 8, exactly: a weight takes part as the number it
-// stands for, with no correction behind the sum, at one instruction more per two
-// weights and rows.  2,048 column confidences, 6 % of them not zero, to 480: 5.5 us,
-// one workgroup's chain; 24,576 numbers to 7 x 480: 22 us for 47 MB, of which the
-// weights' 3.5 instructions are half.
+// stands for.  2,048 column confidences, 6 % of them not zero, to 480: 5.5 us, one
+// workgroup's chain; 24,576 numbers to 7 x 480: 22 us for 47 MB, of which the weights'
+// 4.2 instructions are half.
 #define MV_NT 256
 #define MV_HB 16     // outputs of a half block
 
@@ -398,7 +397,6 @@ struct MvAcc {
     __device__ __forceinline__ void add(uint2 c, float s, const float* x, uint32_t e1032, uint32_t e72) {
         const half2_t k0 = {(_Float16)1032.0f, (_Float16)1032.0f}, k1 = {(_Float16)72.0f, (_Float16)72.0f};
         const uint32_t w[2] = {c.x, c.y};
-        const float m = NX == 1 ? s * x[0] : s;
 #pragma unroll
         for (int k = 0; k < 2; k++) {
             const uint32_t h = w[k] >> 8;
@@ -406,14 +404,10 @@ struct MvAcc {
                                   as_half2(and_or(h, 0x000F000Fu, e1032)) - k0, as_half2(and_or(h, 0x00F000F0u, e72)) - k1};
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float n = (float)(j < 4 ? q[j & 3].x : q[j & 3].y);
-                if (NX == 1) {
-                    v[0][k * 8 + j] = __builtin_fmaf(n, m, v[0][k * 8 + j]);
-                } else {
-                    const float y = __builtin_fmaf(n, m, 0.0f);
+                // (the weight first, exactly: scale * x may overflow or vanish where the weight's product does not)
+                const float y = __builtin_fmaf((float)(j < 4 ? q[j & 3].x : q[j & 3].y), s, 0.0f);
 #pragma unroll
-                    for (int r = 0; r < NX; r++) v[r][k * 8 + j] = __builtin_fmaf(x[r], y, v[r][k * 8 + j]);
-                }
+                for (int r = 0; r < NX; r++) v[r][k * 8 + j] = __builtin_fmaf(x[r], y, v[r][k * 8 + j]);
             }
         }
     }

@@ -78,3 +78,35 @@ def test_a_weight_of_zero_under_a_large_scale(rt):
     r = rt.Readout4(torch.from_numpy(rec).cuda(), n, 1, 40)
     y = r.logits(words(np.ones((3, n), bool)))
     assert torch.all(y == 4 * 2.0 ** -10)
+
+
+def uniform(rt, n, codes, scale):
+    """[1, n, 1, 40] with one scale and `codes` [n]."""
+    rec = np.zeros((1, n, 64), np.uint8)
+    rec[0, :, :32] = (np.asarray(codes) * 0x11)[:, None]
+    rec[0, :, 32:36] = (np.full((n, 2), scale, np.float32).view(np.uint32) >> 16).astype(np.uint16).view(np.uint8)
+    return rt.Readout4(torch.from_numpy(rec).cuda(), n, 1, 40)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 4, 6])
+def test_large_finite_numbers_meet_zero_weights(rt, rows):
+    """scale * x would overflow where x * (scale * (code - 8)) does not: a zero weight adds nothing to a finite x."""
+    n = 70
+    codes = np.full(n, 8)
+    codes[[3, 64]] = 9, 7
+    r = uniform(rt, n, codes, 8.0)
+    x = torch.full((rows, n), 1e38, device="cuda")
+    x[:, 3], x[:, 64] = 3.0, 5.0
+    assert torch.all(r.matvec(x) == 8.0 * 3 - 8.0 * 5)
+    x[:, 10] = -3e38
+    assert torch.all(r.matvec(x) == 8.0 * 3 - 8.0 * 5)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 4])
+def test_small_numbers_keep_their_weights(rt, rows):
+    """scale * x lies below float32's numbers, x * (scale * (code - 8)) does not: 2^-151 * 6 = 1.5 * 2^-149 rounds to
+    2 * 2^-149, not to 0 (one term, so that nothing is rounded twice)."""
+    r = uniform(rt, 33, np.full(33, 14), 2.0 ** -31)
+    x = torch.zeros((rows, 33), device="cuda")
+    x[:, 32] = 2.0 ** -120
+    assert torch.all(r.matvec(x) == 2 * 2.0 ** -149)
