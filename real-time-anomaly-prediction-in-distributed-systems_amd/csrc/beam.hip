@@ -44,24 +44,24 @@ __device__ __forceinline__ double fma_s(double a, double b, double c) {
     return fma(a, b, c);
 }
 
-// exp(x - m) for finite m >= x, x = -infinity included (0): 2^t as 2^n 2^f, |f| <=
-// 1/2, the Taylor series of 2^f to degree 10 (remainder (ln 2 / 2)^11 / 11! =
-// 2e-13).  A beam's sum off by that much moves a float32 score over a rounding
-// border, by one step, once in some 10^6 candidates, as any other order of the
-// same float64 sum does once in 10^9.
+// exp(x - m) for finite m >= x, x = -infinity included (0), to a few units of 2^-53 as
+// any float64 exponential: 2^t as 2^n 2^f, |f| <= 1/2, and 2^f as 1 + f q(f), q the
+// polynomial of degree 10 through (2^f - 1) / f at the 11 Chebyshev nodes (off by 0.2 *
+// 2^-53 with these coefficients).
 __device__ __forceinline__ double exp_diff(float x, double m) {
     const double t = fmax(((double)x - m) * 1.4426950408889634074, -1100.0);
     const double n = rint(t), f = t - n;
-    double p = 7.0549116208011233e-9;       // ln(2)^k / k!, k = 10 ... 1
-    p = fma_s(p, f, 1.0178086009239699e-7);
-    p = fma_s(p, f, 1.3215486790144309e-6);
-    p = fma_s(p, f, 1.5252733804059841e-5);
-    p = fma_s(p, f, 1.5403530393381610e-4);
-    p = fma_s(p, f, 1.3333558146428443e-3);
-    p = fma_s(p, f, 9.6181291076284772e-3);
-    p = fma_s(p, f, 5.5504108664821580e-2);
-    p = fma_s(p, f, 2.4022650695910071e-1);
-    p = fma_s(p, f, 6.9314718055994531e-1);
+    double p = 4.4549605981865186e-10;
+    p = fma_s(p, f, 7.072585949269223e-09);
+    p = fma_s(p, f, 1.0178062445845774e-07);
+    p = fma_s(p, f, 1.321544258792169e-06);
+    p = fma_s(p, f, 1.525273382983612e-05);
+    p = fma_s(p, f, 1.540353044173605e-04);
+    p = fma_s(p, f, 1.3333558146416936e-03);
+    p = fma_s(p, f, 9.618129107606888e-03);
+    p = fma_s(p, f, 5.55041086648216e-02);
+    p = fma_s(p, f, 0.24022650695910097);
+    p = fma_s(p, f, 0.6931471805599453);
     p = fma(p, f, 1.0);
     return ldexp(p, (int)n);
 }
