@@ -38,8 +38,6 @@ def beam_select(logits, scores, beams: int, live=None):
     code = dtype_code(logits.dtype) if isinstance(logits, torch.Tensor) else -1
     if code not in (0, 2, 3) or logits.dim() != 3 or not logits.is_cuda:
         raise ValueError("logits must be a float32, float16 or bfloat16 CUDA tensor [groups, beams_in, n_outputs]")
-    if torch.is_grad_enabled() and logits.requires_grad:
-        raise ValueError("a selection has no gradient: detach the logits")
     groups, win, v = logits.shape
     dev = logits.device
     beams = int(beams)
@@ -49,6 +47,8 @@ def beam_select(logits, scores, beams: int, live=None):
     if not isinstance(scores, torch.Tensor) or scores.dtype != torch.float32 or scores.device != dev or \
             scores.shape != (groups, win):
         raise ValueError("scores must be float32 [groups, beams_in] on %s" % dev)
+    if (logits.requires_grad or scores.requires_grad) and torch.is_grad_enabled():
+        raise ValueError("a selection has no gradient: detach the logits and scores")
     if live is not None and (not isinstance(live, torch.Tensor) or live.dtype != torch.int32 or live.device != dev or
                              live.shape != (groups,)):
         raise ValueError("live must be int32 [groups] on %s" % dev)
@@ -77,8 +77,8 @@ def beam_reorder(buffers, parent, out=None):
     or [groups, beams, ...]; parent: int32 [groups, beams] (a parent outside
     0..beams-1 counts as w itself).  out: tensors like the buffers to write to;
     None reorders in place, and a buffer that stands in `out` as well is
-    reordered in place.  Buffers that overlap otherwise are refused.  Returns
-    the reordered tensors as a list."""
+    reordered in place.  Buffers that overlap otherwise are refused, and so are
+    those that require a gradient.  Returns the reordered tensors as a list."""
     import torch
     L = _lib.lib()
     buffers = list(buffers)
@@ -94,6 +94,7 @@ def beam_reorder(buffers, parent, out=None):
     parent = parent.contiguous()
     n = len(buffers)
     p = [0] * (3 * n)  # sources, destinations, row bytes
+    grad = False
     for k, a in enumerate(buffers):
         b = dst[k]
         if not isinstance(a, torch.Tensor) or a.device != dev or not a.is_contiguous() or b is not a and (
@@ -104,9 +105,13 @@ def beam_reorder(buffers, parent, out=None):
         if not shape or shape[0] != rows and shape[:2] != (groups, beams):
             raise ValueError("a buffer must be [groups * beams, ...] or [groups, beams, ...] for %d groups of %d, got %s" %
                              (groups, beams, tuple(shape)))
+        grad = grad or a.requires_grad or b.requires_grad
         p[k], p[n + k], p[2 * n + k] = a.data_ptr(), b.data_ptr(), a.nbytes // rows if rows else 0
+    if grad and torch.is_grad_enabled():
+        raise ValueError("a reordering has no gradient: detach the buffers")
     p = array.array("Q", p)
     at = p.buffer_info()[0]
     with _On(dev.index) as stream:
         check(L.htm_beam_reorder(n, at, at + 8 * n, at + 16 * n, parent.data_ptr(), groups, beams, stream))
+    torch._C._increment_version(dst)  # (a backward pass that has kept one of them notices)
     return dst

@@ -179,6 +179,9 @@ class Readout4:
         if not isinstance(out, torch.Tensor) or out.dtype != torch.float32 or out.device != self.device or \
                 out.shape != shape or not out.is_contiguous():
             raise ValueError("out must be a contiguous float32 tensor %s on %s" % (shape, self.device))
+        if out.requires_grad and torch.is_grad_enabled():
+            raise ValueError("a frozen read-out has no gradient: detach out")
+        torch._C._increment_version((out,))  # (a backward pass that has kept it notices)
         return out
 
     def _pattern(self, pattern):
