@@ -16,6 +16,7 @@ from .readout import _On, dtype_code
 
 MAX_BEAMS = 64
 MAX_BUFFERS = 32
+MAX_GROUPS = 2 ** 31 - 1
 
 
 def beam_select(logits, scores, beams: int, live=None):
@@ -44,6 +45,8 @@ def beam_select(logits, scores, beams: int, live=None):
     if not 1 <= win <= MAX_BEAMS or not 1 <= beams <= MAX_BEAMS or v < 1 or win * v > 2 ** 30:
         raise ValueError("1..%d beams in and out, n_outputs >= 1 and beams_in * n_outputs <= 2**30 (got %d, %d, %d)" %
                          (MAX_BEAMS, win, beams, v))
+    if groups > MAX_GROUPS:
+        raise ValueError("at most 2**31 - 1 groups (got %d)" % groups)
     if not isinstance(scores, torch.Tensor) or scores.dtype != torch.float32 or scores.device != dev or \
             scores.shape != (groups, win):
         raise ValueError("scores must be float32 [groups, beams_in] on %s" % dev)
@@ -89,6 +92,8 @@ def beam_reorder(buffers, parent, out=None):
     if not 1 <= len(buffers) <= MAX_BUFFERS or len(dst) != len(buffers):
         raise ValueError("1..%d buffers and as many destinations" % MAX_BUFFERS)
     groups, beams = parent.shape
+    if groups > MAX_GROUPS:
+        raise ValueError("at most 2**31 - 1 groups (got %d)" % groups)
     rows = groups * beams
     dev = parent.device
     parent = parent.contiguous()

@@ -741,9 +741,9 @@ static void select_launch(SelArgs a, int32_t groups, void* work, hipStream_t st)
             hipLaunchKernelGGL(beam_chunk_kernel<T>, grid, dim3(256), 0, st, a, k, r0);
         }
     }
-    for (int32_t g0 = 0; g0 < groups; g0 += BS_GROUPS) {
+    for (int64_t g0 = 0; g0 < groups; g0 += BS_GROUPS) {
         a.g0 = g0;
-        const dim3 grid(groups - g0 < BS_GROUPS ? groups - g0 : BS_GROUPS);
+        const dim3 grid((uint32_t)(groups - g0 < BS_GROUPS ? groups - g0 : BS_GROUPS));
         if (small) {
             const int each = (a.win + 15) / 16, waves = each > 2 ? (a.win + 3) / 4 : (a.win + each - 1) / each;
             const auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(waves * 64), waves * 64 * 16, st, a); };

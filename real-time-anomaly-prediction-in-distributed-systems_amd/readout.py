@@ -54,6 +54,14 @@ class _On:
             torch._C._cuda_setDevice(self.before)
 
 
+def _q4_shape(*sizes):
+    """The htm_q4_shape of (n_models, n_inputs, n_heads, n_outputs, group)."""
+    for k in sizes:
+        if not -2 ** 31 <= k < 2 ** 31:
+            raise ValueError("a read-out's sizes are below 2**31 (got %s)" % (sizes,))
+    return _lib.Q4Shape(*sizes)
+
+
 class Readout4:
     """The 4-bit matrices of n_models read-outs, n_inputs x n_heads x
     n_outputs each (heads: the classifier's look-ahead steps).
@@ -71,7 +79,7 @@ class Readout4:
             raise ValueError("records must be a contiguous uint8 CUDA tensor [n_models, n_inputs, record bytes]")
         self.n_models, self.n_inputs = int(records.shape[0]), int(n_inputs)
         self.n_heads, self.n_outputs, self.group = int(n_heads), int(n_outputs), int(group)
-        self._shape = _lib.Q4Shape(self.n_models, self.n_inputs, self.n_heads, self.n_outputs, self.group)
+        self._shape = _q4_shape(self.n_models, self.n_inputs, self.n_heads, self.n_outputs, self.group)
         self._pshape = ctypes.addressof(self._shape)
         per = self._L.htm_q4_record_bytes(self._pshape)
         if not per:
@@ -92,7 +100,7 @@ class Readout4:
     def record_bytes(cls, n_models: int, n_inputs: int, n_heads: int, n_outputs: int, group: int = 32) -> int:
         """Bytes of one input's record."""
         L = _lib.lib()
-        s = _lib.Q4Shape(int(n_models), int(n_inputs), int(n_heads), int(n_outputs), int(group))
+        s = _q4_shape(int(n_models), int(n_inputs), int(n_heads), int(n_outputs), int(group))
         per = L.htm_q4_record_bytes(ctypes.addressof(s))
         if not per:
             raise ValueError(L.htm_last_error().decode(errors="replace"))
@@ -165,6 +173,8 @@ class Readout4:
         if x.dim() != 2 or x.shape[1] != width:
             raise ValueError("%s must be [rows, %d], got %s" % (what, width, tuple(x.shape)))
         n = x.shape[0]
+        if n >= 2 ** 31:
+            raise ValueError("too many rows: %d" % n)
         if n % self.n_models:
             raise ValueError("%d rows do not divide over %d models" % (n, self.n_models))
         if (x.stride(1) != 1 and width > 1) or (n > 1 and x.stride(0) < width):
