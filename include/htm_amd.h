@@ -464,7 +464,7 @@ int htm_cls_import_state(htm_classifier* cls, int32_t region, int32_t stream_beg
  * Records: uint8 [n_models][n_inputs][htm_q4_record_bytes], one input's weights:
  * per head the codes of its outputs (padded to a multiple of 32; the lower half
  * of a byte first), then per head ceil(padded / group) scales; padding is
- * ignored; scales are 0 or within 2^-110 .. 2^100.  Base address and d_x / d_pattern /
+ * ignored; scales are 0 or of a size within 2^-110 .. 2^100 (htm_q4_check).  Base address and d_x / d_pattern /
  * d_out as the element type asks, records 16-byte aligned; d_out and d_work overlap
  * nothing else of the call. */
 typedef struct {
@@ -493,6 +493,9 @@ int htm_q4_quantise(const htm_q4_shape* shape, const void* d_weights, int32_t dt
  * counts (maxBucketIdx + 1). */
 int htm_cls_quantise(const htm_classifier* cls, int32_t stream_begin, int32_t step_begin, const htm_q4_shape* shape,
                      void* d_records, int32_t* d_live, int32_t* d_bad, void* stream);
+/* *d_bad (DEVICE int32, zeroed by the caller) is set to 1 if a scale of the records is
+ * out of its range, infinite or NaN: products with it are undefined. */
+int htm_q4_check(const htm_q4_shape* shape, const void* d_records, int32_t* d_bad, void* stream);
 /* y for word bitmaps: d_pattern DEVICE uint32, row r at r * pattern_stride words
  * (n_inputs / 32 of them used; bit b of word w is input 32 w + b).  d_out: float
  * [n_rows][n_heads][n_outputs]. */

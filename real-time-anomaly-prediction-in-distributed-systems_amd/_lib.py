@@ -126,7 +126,7 @@ EXPORTED = [
     "htm_likelihood_create", "htm_likelihood_destroy", "htm_likelihood_step",
     "htm_cls_create", "htm_cls_destroy", "htm_cls_compute", "htm_cls_status", "htm_cls_state_bytes",
     "htm_cls_export_state", "htm_cls_import_state", "htm_cls_quantise",
-    "htm_q4_record_bytes", "htm_q4_quantise", "htm_q4_logits", "htm_q4_probabilities", "htm_q4_work_bytes", "htm_q4_matvec",
+    "htm_q4_record_bytes", "htm_q4_quantise", "htm_q4_check", "htm_q4_logits", "htm_q4_probabilities", "htm_q4_work_bytes", "htm_q4_matvec",
     "htm_beam_work_bytes", "htm_beam_select", "htm_beam_reorder", "htm_reorder_streams", "htm_copy_streams",
 ]
 
@@ -222,6 +222,7 @@ def lib():
     L.htm_q4_record_bytes.argtypes = [vp]
     L.htm_q4_record_bytes.restype = sz
     L.htm_q4_quantise.argtypes = [vp, vp, i32, i64, i64, i64, vp, vp, vp]
+    L.htm_q4_check.argtypes = [vp, vp, vp, vp]
     L.htm_q4_logits.argtypes = [vp, vp, vp, i64, i32, vp, vp]
     L.htm_q4_probabilities.argtypes = [vp, vp, vp, i64, vp, i32, vp, vp]
     L.htm_q4_work_bytes.argtypes = [vp, i32]

@@ -124,6 +124,20 @@ int q4_quantise_launch(const Q4Dims& d, const void* w, int32_t dtype, int64_t ms
     return hipGetLastError() == hipSuccess ? HTM_OK : htm_fail(HTM_E_HIP, "q4 quantise launch failed");
 }
 
+// *bad = 1 if a record's scale is neither 0 nor within its range: a thread per scale, neighbours side by side.  256 x
+// 24,576 records of 105 scales: 0.6 ms.
+__global__ void __launch_bounds__(Q4_NT) q4_check_kernel(Q4Dims d, const uint8_t* __restrict__ rec, int32_t* bad) {
+    const int per = d.nh * d.ngrp;
+    const int64_t total = (int64_t)d.nm * d.ni * per;
+    bool odd = false;
+    for (int64_t i = (int64_t)blockIdx.x * Q4_NT + threadIdx.x; i < total; i += (int64_t)gridDim.x * Q4_NT) {
+        const int64_t row = i / per;
+        const uint16_t b = reinterpret_cast<const uint16_t*>(rec + row * d.pitch + d.scales)[i - row * per] & 0x7FFFu;
+        odd |= b && (b < (uint16_t)((127 - 110) << 7) || b > (uint16_t)((127 + 100) << 7));
+    }
+    if (odd) *bad = 1;
+}
+
 // ------------------------------------------------------------------ products
 // A record's block: 32 outputs' codes in 16 bytes, under one scale.  A code's four
 // bits are masked where they lie, under the exponent that makes the lowest of them
@@ -828,6 +842,17 @@ int htm_q4_quantise(const htm_q4_shape* s, const void* w, int32_t dtype, int64_t
     if (!w || !bad || (dtype != HTM_T_F32 && dtype != HTM_T_F64) || ms < 0 || is < 0 || hs < 0)
         return htm_fail(HTM_E_INVALID, "%s: invalid argument", __func__);
     return q4_quantise_launch(d, w, dtype, ms, is, hs, rec, bad, (hipStream_t)stream);
+}
+
+int htm_q4_check(const htm_q4_shape* s, const void* rec, int32_t* bad, void* stream) {
+    Q4Dims d;
+    if (int r = q4_dims(s, __func__, &d)) return r;
+    if (int r = q4_aligned(rec, __func__)) return r;
+    if (!bad) return htm_fail(HTM_E_INVALID, "%s: invalid argument", __func__);
+    const int64_t blocks = ((int64_t)d.nm * d.ni * d.nh * d.ngrp + Q4_NT - 1) / Q4_NT;
+    hipLaunchKernelGGL(q4_check_kernel, dim3((uint32_t)std::min<int64_t>(blocks, 16384)), dim3(Q4_NT), 0, (hipStream_t)stream, d,
+                       (const uint8_t*)rec, bad);
+    return hipGetLastError() == hipSuccess ? HTM_OK : htm_fail(HTM_E_HIP, "q4 check launch failed");
 }
 
 static int q4_bitmap(const htm_q4_shape* s, const void* rec, const uint32_t* pat, int64_t ps, int32_t n_rows,

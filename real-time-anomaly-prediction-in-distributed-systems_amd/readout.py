@@ -68,10 +68,12 @@ class Readout4:
 
     `records`: uint8 CUDA tensor [n_models, n_inputs, record bytes] in the
     layout of htm_q4_shape (include/htm_amd.h); `quantize`, `from_classifier`
-    and `SDRClassifier.readout4` make it.  `live`: optional int32 [n_models],
+    and `SDRClassifier.readout4` make it.  Its scales must be 0 or of a size
+    within 2**-110 .. 2**100; others raise ValueError (the check waits for the
+    device, and is left out while a graph is captured).  `live`: optional int32 [n_models],
     how many of a head's outputs are in use (`probabilities`' default)."""
 
-    def __init__(self, records, n_inputs: int, n_heads: int, n_outputs: int, group: int = 32, live=None):
+    def __init__(self, records, n_inputs: int, n_heads: int, n_outputs: int, group: int = 32, live=None, *, _new=False):
         import torch
         self._L = _lib.lib()
         if not isinstance(records, torch.Tensor) or records.dtype != torch.uint8 or records.dim() != 3 or \
@@ -94,6 +96,12 @@ class Readout4:
         self._index = records.device.index
         self._rec = records.data_ptr()
         self.live = None if live is None else self._live(live)
+        if not _new and not torch.cuda.is_current_stream_capturing():
+            with _On(self._index) as stream:
+                bad = torch.zeros(1, dtype=torch.int32, device=self.device)
+                check(self._L.htm_q4_check(self._pshape, self._rec, bad.data_ptr(), stream))
+                if bad.item():
+                    raise ValueError("the records' scales must be 0 or of a size within 2**-110 .. 2**100")
 
     # ------------------------------------------------------------- making one
     @classmethod
@@ -123,7 +131,7 @@ class Readout4:
         with _On(w.device.index) as stream:
             rec = torch.zeros((nm, ni, per), dtype=torch.uint8, device=w.device)
             bad = torch.zeros(1, dtype=torch.int32, device=w.device)
-            self = cls(rec, ni, nh, no, group, live)
+            self = cls(rec, ni, nh, no, group, live, _new=True)
             check(self._L.htm_q4_quantise(self._pshape, w.data_ptr(), dtype_code(w.dtype), w.stride(0), w.stride(1),
                                           w.stride(2), self._rec, bad.data_ptr(), stream))
             if bad.item():
@@ -151,7 +159,7 @@ class Readout4:
             rec = torch.zeros((n, classifier.n_inputs, per), dtype=torch.uint8, device=dev)
             live = torch.empty(n, dtype=torch.int32, device=dev)
             bad = torch.zeros(1, dtype=torch.int32, device=dev)
-            self = cls(rec, classifier.n_inputs, nh, classifier.n_buckets, group, live)
+            self = cls(rec, classifier.n_inputs, nh, classifier.n_buckets, group, live, _new=True)
             check(self._L.htm_cls_quantise(classifier.h, int(s0), y0, self._pshape, self._rec, live.data_ptr(),
                                            bad.data_ptr(), stream))
             if bad.item():
@@ -229,7 +237,9 @@ class Readout4:
         """y of vectors of numbers [rows, n_inputs], float32 / float16 /
         bfloat16 (the engine's "col_confidence", an averaged activity).  An
         infinite number makes its row's outputs infinite (NaN where the weight
-        is zero), a NaN makes them NaN; other rows keep theirs."""
+        is zero), a NaN makes them NaN; other rows keep theirs.  With five and
+        more rows a matrix, what lies below 2**-126 in a number's 8-bit parts,
+        a product or a sum may count as zero."""
         import torch
         if not isinstance(x, torch.Tensor) or dtype_code(x.dtype) not in (0, 2, 3):
             raise ValueError("x must be a float32, float16 or bfloat16 tensor [rows, n_inputs]")
