@@ -189,7 +189,7 @@ class Readout4:
             x = x.contiguous()
         return x, n, x.stride(0)
 
-    def _out(self, out, n):
+    def _out(self, out, n, *reads):
         import torch
         shape = (n, self.n_heads, self.n_outputs)
         if out is None:
@@ -199,6 +199,12 @@ class Readout4:
             raise ValueError("out must be a contiguous float32 tensor %s on %s" % (shape, self.device))
         if out.requires_grad and torch.is_grad_enabled():
             raise ValueError("a frozen read-out has no gradient: detach out")
+        o0 = out.data_ptr()
+        for t in (self.records, *reads):  # (a workgroup writes while others still read)
+            if t is not None and t.numel():
+                size = sum((k - 1) * s for k, s in zip(t.shape, t.stride())) + 1
+                if t.data_ptr() < o0 + out.nbytes and o0 < t.data_ptr() + size * t.element_size():
+                    raise ValueError("out overlaps what the call reads")
         torch._C._increment_version((out,))  # (a backward pass that has kept it notices)
         return out
 
@@ -214,9 +220,10 @@ class Readout4:
     def logits(self, pattern, out=None):
         """y [rows, n_heads, n_outputs] float32 of word bitmaps [rows,
         n_inputs / 32] (the engine's "tm_output"): bit b of word w is input
-        32 w + b.  A row without a set bit gives zeros."""
+        32 w + b.  A row without a set bit gives zeros.  out (of every product):
+        a contiguous tensor to write to, apart from all that the call reads."""
         p, n, stride = self._pattern(pattern)
-        y = self._out(out, n)
+        y = self._out(out, n, p)
         with _On(self._index) as stream:
             check(self._L.htm_q4_logits(self._pshape, self._rec, p.data_ptr(), stride, n, y.data_ptr(), stream))
         return y
@@ -227,7 +234,7 @@ class Readout4:
         classifier region's "probabilities".  n_outputs <= 1024."""
         p, n, stride = self._pattern(pattern)
         lv = self.live if live is None else self._live(live)
-        y = self._out(out, n)
+        y = self._out(out, n, p, lv)
         with _On(self._index) as stream:
             check(self._L.htm_q4_probabilities(self._pshape, self._rec, p.data_ptr(), stride,
                                                lv.data_ptr() if lv is not None else None, n, y.data_ptr(), stream))
@@ -246,7 +253,7 @@ class Readout4:
         if x.requires_grad and torch.is_grad_enabled():
             raise ValueError("a frozen read-out has no gradient: detach x")
         v, n, stride = self._rows(x, self.n_inputs, "x")
-        y = self._out(out, n)
+        y = self._out(out, n, v)
         nb = self._L.htm_q4_work_bytes(self._pshape, n)
         with _On(self._index) as stream:
             work = torch.empty(nb, dtype=torch.uint8, device=self.device) if nb else None
