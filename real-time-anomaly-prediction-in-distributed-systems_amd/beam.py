@@ -17,6 +17,7 @@ from .readout import _On, dtype_code
 MAX_BEAMS = 64
 MAX_BUFFERS = 32
 MAX_GROUPS = 2 ** 31 - 1
+_WHOLE = None  # dtypes of whole numbers and bits: never a view still to be conjugated or negated
 
 
 def beam_select(logits, scores, beams: int, live=None):
@@ -55,11 +56,12 @@ def beam_select(logits, scores, beams: int, live=None):
     if live is not None and (not isinstance(live, torch.Tensor) or live.dtype != torch.int32 or live.device != dev or
                              live.shape != (groups,)):
         raise ValueError("live must be int32 [groups] on %s" % dev)
+    logits = logits.resolve_neg()
     gs, bs, vs = logits.stride()
     if vs != 1 and v > 1:
         logits = logits.contiguous()
         gs, bs, _ = logits.stride()
-    scores = scores.contiguous()
+    scores = scores.resolve_neg().contiguous()
     live = live.contiguous() if live is not None else None
     with _On(dev.index) as stream:
         o_score, o_parent, o_bucket = scores.new_empty((3, groups, beams), dtype=torch.int32).unbind(0)
@@ -83,6 +85,9 @@ def beam_reorder(buffers, parent, out=None):
     reordered in place.  Buffers that overlap otherwise are refused, and so are
     those that require a gradient.  Returns the reordered tensors as a list."""
     import torch
+    global _WHOLE
+    if _WHOLE is None:
+        _WHOLE = {torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64, torch.bool}
     L = _lib.lib()
     buffers = list(buffers)
     dst = buffers if out is None else list(out)
@@ -100,17 +105,23 @@ def beam_reorder(buffers, parent, out=None):
     n = len(buffers)
     p = [0] * (3 * n)  # sources, destinations, row bytes
     grad = False
+    index, tensor = dev.index, torch.Tensor
     for k, a in enumerate(buffers):
         b = dst[k]
-        if not isinstance(a, torch.Tensor) or a.device != dev or not a.is_contiguous() or b is not a and (
-                not isinstance(b, torch.Tensor) or b.device != dev or b.dtype != a.dtype or b.shape != a.shape or
-                not b.is_contiguous()):
+        ok = isinstance(a, tensor) and a.get_device() == index and a.is_contiguous()
+        if ok:
+            shape = a.shape
+            grad = grad or a.requires_grad
+        if ok and b is not a:
+            ok = isinstance(b, tensor) and b.get_device() == index and b.dtype is a.dtype and b.shape == shape and b.is_contiguous()
+            if ok:
+                grad = grad or b.requires_grad
+                ok = a.dtype in _WHOLE or a.is_conj() == b.is_conj() and a.is_neg() == b.is_neg()
+        if not ok:
             raise ValueError("buffers and destinations must be contiguous, alike, and on %s" % dev)
-        shape = a.shape
         if not shape or shape[0] != rows and shape[:2] != (groups, beams):
             raise ValueError("a buffer must be [groups * beams, ...] or [groups, beams, ...] for %d groups of %d, got %s" %
                              (groups, beams, tuple(shape)))
-        grad = grad or a.requires_grad or b.requires_grad
         p[k], p[n + k], p[2 * n + k] = a.data_ptr(), b.data_ptr(), a.nbytes // rows if rows else 0
     if grad and torch.is_grad_enabled():
         raise ValueError("a reordering has no gradient: detach the buffers")

@@ -123,6 +123,7 @@ class Readout4:
         if not isinstance(weights, torch.Tensor) or not weights.is_cuda or weights.dim() != 4 or \
                 weights.dtype not in (torch.float32, torch.float64):
             raise ValueError("weights must be a float32 or float64 CUDA tensor [n_models, n_inputs, n_heads, n_outputs]")
+        weights = weights.resolve_neg()
         w = weights if weights.stride(3) == 1 or weights.shape[3] == 1 else weights.contiguous()
         if min(w.stride()[:3]) < 0:
             w = w.contiguous()
@@ -185,6 +186,7 @@ class Readout4:
             raise ValueError("too many rows: %d" % n)
         if n % self.n_models:
             raise ValueError("%d rows do not divide over %d models" % (n, self.n_models))
+        x = x.resolve_neg()
         if (x.stride(1) != 1 and width > 1) or (n > 1 and x.stride(0) < width):
             x = x.contiguous()
         return x, n, x.stride(0)
@@ -195,7 +197,7 @@ class Readout4:
         if out is None:
             return self.records.new_empty(shape, dtype=torch.float32)
         if not isinstance(out, torch.Tensor) or out.dtype != torch.float32 or out.device != self.device or \
-                out.shape != shape or not out.is_contiguous():
+                out.shape != shape or not out.is_contiguous() or out.is_neg():
             raise ValueError("out must be a contiguous float32 tensor %s on %s" % (shape, self.device))
         if out.requires_grad and torch.is_grad_enabled():
             raise ValueError("a frozen read-out has no gradient: detach out")
