@@ -544,11 +544,12 @@ int htm_beam_reorder(int32_t n_buffers, const void* const* d_src, void* const* d
  * place: stream g * n_beams + w goes on as its parent d_parent[g][w] would have.
  * n_streams must be a multiple of n_beams.  Error flags (htm_tm_header.error) stay with
  * their stream and its parent's are added: htm_status reports what any stream ran
- * into, also where that stream's state has since been replaced. */
+ * into, also where that stream's state has since been replaced.  Not while `stream`
+ * is captured into a graph (HTM_E_STATE): what moves depends on the calls before. */
 int htm_reorder_streams(htm_engine* eng, const int32_t* d_parent, int32_t n_beams, void* stream);
 /* Stream s of fleet dst goes on as stream d_index[s] (DEVICE int32 [n_streams of
  * dst], 0..n_streams of src - 1; others leave s as it is) of fleet src: a fork.  Error
- * flags as above.
+ * flags and captures as above.
  * Both are fleets of one model (htm_model_id) and configuration on one device; others
  * are refused; dst != src. */
 int htm_copy_streams(htm_engine* dst, htm_engine* src, const int32_t* d_index, void* stream);

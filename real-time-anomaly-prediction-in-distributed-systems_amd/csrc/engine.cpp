@@ -1770,11 +1770,21 @@ static int after_flush(htm_engine* e, hipStream_t st) {
     return HTM_OK;
 }
 
+// Which form of colConfidence moves, and whether a flush is waited for, are decided
+// here at the call: a replay would repeat what held when it was captured.
+static int not_captured(hipStream_t st) {
+    hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(st, &s) == hipSuccess && s != hipStreamCaptureStatusNone)
+        return htm_fail(HTM_E_STATE, "a fleet's streams are not moved by a captured graph");
+    return HTM_OK;
+}
+
 int htm_reorder_streams(htm_engine* e, const int32_t* d_parent, int32_t n_beams, void* stream) {
     if (!e || !d_parent) return htm_fail(HTM_E_INVALID, "bad arguments");
     if (!e->fleet) return htm_fail(HTM_E_STATE, "streams of an ordinary engine have models of their own: reorder a fleet");
     if (n_beams < 1 || n_beams > 64 || e->n % n_beams)
         return htm_fail(HTM_E_INVALID, "n_beams must be 1..64 and divide the %d streams", e->n);
+    if (int r = not_captured((hipStream_t)stream)) return r;
     if (int r = after_flush(e, (hipStream_t)stream)) return r;
     RowMoves m;
     stream_rows(e, m);
@@ -1797,6 +1807,7 @@ int htm_copy_streams(htm_engine* dst, htm_engine* src, const int32_t* d_index, v
     if (dst->keep_overlaps != src->keep_overlaps || dst->keep_prev != src->keep_prev)
         return htm_fail(HTM_E_INVALID, "the fleets retain different outputs (HTM_OPT_KEEP_*)");
     hipStream_t st = (hipStream_t)stream;
+    if (int r = not_captured(st)) return r;
     if (int r = after_flush(dst, st)) return r;
     // (one of the two stepped since its colConfidence was last made dense)
     if (dst->conf_packed != src->conf_packed) {

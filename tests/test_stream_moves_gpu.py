@@ -144,3 +144,27 @@ def test_fleets_of_one_model_are_not(rt, model, traces, tmp_path):
     assert b.model_id() in ids
     a.copy_streams(b, index)
     a.status()
+
+
+def test_moves_are_not_captured(rt, model):
+    """The state's form when a move is called decides what moves; a replay would not know it."""
+    fl, src = rt.HTMEngine.fleet(model, 4, q_capacity=4096), rt.HTMEngine.fleet(model, 2, q_capacity=4096)
+    step(fl, 30), step(src, 40)
+    p = torch.tensor([[1, 0], [1, 1]], dtype=torch.int32, device="cuda")
+    i = torch.zeros(4, dtype=torch.int32, device="cuda")
+    before = fl.export_state("tm_bitmaps")
+    x = torch.ones(8, device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        x.mul_(2.0)
+        for move in (lambda: fl.reorder_streams(p), lambda: fl.copy_streams(src, i)):
+            with pytest.raises(rt.HtmError, match="captured"):
+                move()
+    for k in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.all(x == 2.0 ** (k + 1))
+    assert np.array_equal(fl.export_state("tm_bitmaps"), before)
+    fl.reorder_streams(p)
+    assert np.array_equal(fl.export_state("tm_bitmaps"), before[[1, 0, 3, 3]])
