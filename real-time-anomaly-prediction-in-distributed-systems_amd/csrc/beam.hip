@@ -228,7 +228,7 @@ __device__ __forceinline__ void put_rest(const SelArgs& a, int64_t g, int taken)
 // largest, E exponentials, the sum, a logarithm, the scores.  Measured, us, 8 x
 // 480 -> 8: one group 5.6 (the logits in LDS, between barriers: 10.4), 512 groups
 // 8.2 (13.6), 4,096 groups 30 to 34 (54); two beams a wave 7.0, 9.0, 33.  Many groups
-// are bound by instructions, most of them float64: 1.7e7 of a wave, 500 for each
+// are bound by instructions, most of them float64: 1.7e7 of a wave, 510 for each
 // beam, are 31 us of issue at the 4.5 cycles that one takes; the 63 MB take 13.
 template <typename T, int R, int E>
 __global__ void __launch_bounds__(1024) beam_small_kernel(SelArgs a) {

@@ -572,7 +572,8 @@ __global__ void __launch_bounds__(MV_NT, NX == 4 ? 3 : 4)
 
 // Several rows at once, by matrix instructions.  v_mfma_f32_16x16x32_bf16 takes 16
 // rows' numbers for 32 inputs (A) and those inputs' weights of 16 outputs (B).  A
-// weight scale * (code - 8) has 8 + 4 bits, too many for a bfloat16: the scale's
+// weight scale * (code - 8) has up to 11 bits, too many for a bfloat16 (a float16 would
+// hold them, but not the range of all scales): the scale's
 // upper and lower four bits make two bfloat16 products that are exact, and a
 // number takes one (bfloat16), two (float16) or three (float32) bfloat16 parts,
 // so that every product in the sum is exact and only float32 sums round, as in the
@@ -893,7 +894,7 @@ static int q4_raise_lds(const void* kernel, size_t lds, std::atomic<uint64_t>& r
 //   16, 24,576, 7 x 480                            76        35
 //   8, 24,576, 480                                 16        14
 //   12, 4,000, 7 x 480                             22        14
-//   8, 24,576 with 6 % not zero, 7 x 480           14        18
+//   8, 24,576 with 6 % not zero, 7 x 480           14        18 (how many are zero is not known here)
 // and for the first two columns, runs x ranges: 8, 24,576, 7 x 480: 7 x 73 44, 7 x
 // 36 50, 4 x 64 58; 1, 4,000, 480: 2 x 16 9.3, 30 x 1 12.5.  In one launch while a
 // tile holds the inputs (Python call included; in two it takes 12.4): 1, 2,048, 480 8.8;
@@ -963,20 +964,22 @@ static int mv_launch(const MvPlan& p, const Q4Dims& d, const void* rec, const vo
 // How a row's blocks are shared out: runs of at most 64 blocks, or the whole
 // record (up to 512) where no two rows share a matrix and every record comes
 // from memory once; shorter runs until the chip's 256 CUs have a workgroup each.
-// Measured, us (runs x threads; 24,576 inputs, 480 outputs a head):
-//   4,096 rows of one matrix, 1 head: 1 x 256 103, 1 x 512 117, 2 x 256 113
-//   1,024 rows, 7 heads: 2 x 512 207, 1 x 1,024 239, 7 x 256 287
-//   256 rows of own matrices, 7 heads: 1 x 1,024 88, 2 x 512 96, 3 x 256 95
-//   64 rows, 7 heads: 4 x 512 28, 2 x 512 46, 1 x 1,024 74
-//   1 row, 7 heads: 105 x 256 8.9, 21 x 512 10.1, 105 x 1,024 12.6
+// Measured, us (runs x threads; 480 outputs a head, patterns of 768 columns x 32 cells):
+//   4,096 rows of one matrix, 1 head: 1 x 256 109, 1 x 512 132, 2 x 256 124
+//   1,024 rows, 7 heads: 2 x 512 220, 1 x 1,024 262, 7 x 256 294
+//   256 rows of own matrices, 7 heads: 1 x 1,024 84, 2 x 512 87, 3 x 256 88
+//   64 rows, 7 heads: 4 x 512 28, 2 x 512 47, 1 x 1,024 78
+//   1 row, 7 heads: 105 x 256 7.6, 21 x 512 7.9, 105 x 1,024 10.6
+// and of 2,048 x 12, in the same order: 58, 82, 79; 99, 128, 135; 37, 39, 40; 15, 22, 35;
+// 8.1, 9.5, 11.5.
 template <bool SOFTMAX>
 static int q4_rows_launch(const Q4Dims& d, const void* rec, const uint32_t* pat, int64_t ps, int32_t n_rows, int per,
                           const int32_t* live, float* out, hipStream_t st) {
     const int total = d.nh * d.nblk;
     int cblk;
     if (SOFTMAX) {
-        // whole heads, as many as leave the chip's CUs a workgroup each (24,576 inputs, 7 x 480, us: 36 rows 1 head 14.5,
-        // 2 16.1, 4 23.8; 128 rows 30.3, 25.5, 25.3)
+        // whole heads, as many as leave the chip's CUs a workgroup each (2,048 x 12 cells, 7 x 480, us: 36 rows 1 head 14.3,
+        // 2 16.4, 4 25.1; 128 rows 28.2, 25.4, 25.9)
         const int64_t heads = ((int64_t)n_rows * d.nh + 255) / 256;
         cblk = d.nblk * (int)std::max<int64_t>(1, std::min<int64_t>(heads, std::min(d.nh, 64 / d.nblk)));
     } else {
@@ -1020,8 +1023,8 @@ int htm_q4_probabilities(const htm_q4_shape* s, const void* rec, const uint32_t*
     if (d.nblk <= 4 || (int64_t)n_rows * d.nh >= (d.nblk <= 16 ? 100 : 256))
         return q4_rows_launch<true>(d, rec, pat, ps, n_rows, per, live, out, st);
     // too few heads to fill the chip: the products in shorter runs, then the softmax.  One launch and two, us, Python call
-    // included: 64 rows, 65,536 inputs, 1,000 outputs 29 and 19; 255 rows 31 and 33; 24,576 inputs, 480 outputs, 16 rows
-    // 12.7 and 11.6, 128 rows 12.8 and 13.9; 100 outputs, 4 rows 9.3 and 10.8
+    // included: 64 rows, 65,536 inputs, 1,000 outputs 30 and 19; 255 rows 32 and 34; 2,048 x 12 cells, 480 outputs, 16 rows
+    // 13.0 and 12.2, 128 rows 13.1 and 14.2; 768 x 32 cells, 100 outputs, 4 rows 12.6 and 12.0
     if (int r = q4_rows_launch<false>(d, rec, pat, ps, n_rows, per, nullptr, out, st)) return r;
     const int64_t k = (int64_t)n_rows * d.nh;
     hipLaunchKernelGGL(q4_softmax_kernel, dim3((uint32_t)((k + Q4_NT / 64 - 1) / (Q4_NT / 64))), dim3(Q4_NT), 0, st, d, live,
